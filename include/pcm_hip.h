@@ -468,6 +468,105 @@ int pcm_pack_segmented(const float* src_base, void* dst_base, const pcm_pack_des
 int pcm_cast_f32_bf16(const float* x, void* y, long n, void* stream);
 int pcm_cast_bf16_f32(const void* x, float* y, long n, void* stream);
 
+/* ---- alignment of the distilled student (abi >= 6): preference losses, clipped policy loss, transition log-probability, gradient norm ----
+ * Element formats of these calls are named per call and do not depend on the build's 16-bit format.  Elements are formed in fp32, sums are
+ * carried in fp64 in a fixed order (no atomics): results are bitwise the same run to run.  `workspace` is 8-byte aligned caller scratch of at
+ * least the matching *_workspace_bytes; it is only used between the launches of the call.  Gradients are those of grad_scale * loss. */
+#define PCM_DT_F32 0
+#define PCM_DT_BF16 1
+#define PCM_DT_F16 2
+/* log-probability of a noisy sampler transition, x ~ N(mean, std^2) per row:
+ *   logp[b] = -1/2 sum_i ((x - mean) / std[b])^2 - n log std[b] - n/2 log 2 pi,   divided by n with mean_reduce
+ * x, mean [rows][n] contiguous, std fp32 [rows] > 0, logp fp32 [rows].  The gradient by mean: dlogp[b] * (x - mean) / std[b]^2 (/ n). */
+size_t pcm_transition_logprob_workspace_bytes(long rows, long n);
+int pcm_transition_logprob(const void* x, const void* mean, const float* std, int dtype, int mean_reduce, float* logp, long rows, long n,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int pcm_transition_logprob_bwd(const void* x, const void* mean, const float* std, const float* dlogp, int dtype, int mean_reduce, void* dmean,
+                               long rows, long n, void* stream);
+/* Preference losses over pairs.  Rows 0 .. pairs-1 are the preferred samples, rows pairs .. 2 pairs - 1 the rejected ones; log_ratio[row] is the
+ * row's log ratio of policy and reference and s = beta * (log_ratio[p] - log_ratio[pairs + p]) the pair's margin.
+ *   SIGMOID  -(1 - e) log sig(s) - e log sig(-s)  (e = label_smoothing);   HINGE  max(0, 1 - s);   SQUARE  (s / beta - 1 / (2 beta))^2
+ * loss[0] is the mean over the pairs.  loss fp32 [1], log_ratio fp32 [2 pairs]. */
+#define PCM_PAIR_SIGMOID 0
+#define PCM_PAIR_HINGE 1
+#define PCM_PAIR_SQUARE 2
+/* log ratio from denoising errors: log_ratio[r] = -w[r] k sum_i ((target - pred)^2 - (target - ref)^2), k = 1 / n (mean_reduce) or 1.
+ * pred, ref, target, dpred [2 pairs][n] contiguous in `dtype`. */
+typedef struct {
+  const void *pred, *ref, *target;
+  const float* weight; /* [2 pairs] or NULL: 1 */
+  void* dpred;         /* NULL: no gradient */
+  float *loss, *log_ratio;
+  void* workspace;
+  size_t workspace_bytes;
+  long pairs, n;
+  double beta, label_smoothing, grad_scale;
+  int dtype, kind, mean_reduce;
+} pcm_denoise_preference_args;
+size_t pcm_denoise_preference_loss_workspace_bytes(long pairs, long n);
+int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a, void* stream);
+/* log ratio from log-probabilities of tokens or sampler steps: the sum (mean with mean_reduce; 0 for a row without places) of logp - ref_logp over
+ * the places that count: mask[row][col] != 0 and col < lengths[row] (lengths are clamped to [0, cols]).  Values in other places are not used
+ * and their gradient is 0.  Rows may be strided (ld_* >= cols, unit inner stride). */
+typedef struct {
+  const void *logp, *ref_logp;
+  const unsigned char* mask; /* or NULL */
+  const void* lengths;       /* int32 / int64 [2 pairs] or NULL */
+  void* dlogp;               /* NULL: no gradient */
+  float *loss, *log_ratio;
+  void* workspace;
+  size_t workspace_bytes;
+  long pairs, cols, ld_logp, ld_ref, ld_mask, ld_dlogp;
+  double beta, label_smoothing, grad_scale;
+  int dtype, kind, mean_reduce, lengths_i64;
+} pcm_preference_args;
+size_t pcm_preference_loss_workspace_bytes(long pairs, long cols);
+int pcm_preference_loss(const pcm_preference_args* a, void* stream);
+/* Clipped policy loss with a KL term.  Per place that counts (mask / lengths as above), r = exp(logp - old_logp), d = ref_logp - logp:
+ *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)  +  kl_coef * (exp(d) - d - 1)
+ * old_logp NULL: the policy itself (r = 1 with its gradient).  A = advantages[row] (adv_per_row) or advantages[row][col].
+ * Reduced by TOKEN: mean over all places;  ROW: mean over the rows of each row's mean (a row without places adds 0);  SUM.
+ * stats fp32 [4] = {clipped objective, KL} (reduced the same way; loss = objective + kl_coef * KL), share of places held by the clip, places. */
+#define PCM_POLICY_TOKEN 0
+#define PCM_POLICY_ROW 1
+#define PCM_POLICY_SUM 2
+typedef struct {
+  const void *logp, *old_logp, *ref_logp;
+  const float* advantages;
+  const unsigned char* mask;
+  const void* lengths;
+  void* dlogp;
+  float *loss, *stats;
+  void* workspace;
+  size_t workspace_bytes;
+  long rows, cols, ld_logp, ld_old, ld_ref, ld_adv, ld_mask, ld_dlogp;
+  double clip_low, clip_high, kl_coef, grad_scale;
+  int dtype, reduce, adv_per_row, lengths_i64;
+} pcm_policy_args;
+size_t pcm_policy_loss_workspace_bytes(long rows, long cols);
+int pcm_policy_loss(const pcm_policy_args* a, void* stream);
+/* Global norm of gradients held in many tensors, and their clipping (torch.nn.utils' rule, as in pcm_adamw_clip_step):
+ *   sumsq = sum g^2 (fp64), norm = sqrt(sumsq);   dst = src * min(1, max_norm / (norm + 1e-6))
+ * descs / chunks are tables in DEVICE memory: tensor t is descs[t] and is cut into chunks {t, start} with start = 0, PCM_GRAD_CHUNK, ... < n.
+ * dst may be src (then nothing is written when nothing has to be clipped) or a tensor apart; its format may be another one.
+ * sumsq is what pcm_adamw_clip_step takes as gradsq. */
+#define PCM_GRAD_CHUNK 16384
+typedef struct {
+  const void* src;
+  void* dst;
+  long n;
+  int src_dtype, dst_dtype;
+} pcm_grad_desc;
+typedef struct {
+  long start;
+  long tensor;
+} pcm_grad_chunk;
+size_t pcm_grad_norm_workspace_bytes(int nchunks);
+int pcm_grad_norm(const pcm_grad_desc* descs, const pcm_grad_chunk* chunks, int nchunks, float* norm, double* sumsq, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int pcm_grad_clip(const pcm_grad_desc* descs, const pcm_grad_chunk* chunks, int nchunks, double max_norm, float* norm, double* sumsq,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

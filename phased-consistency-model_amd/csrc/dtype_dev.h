@@ -1,0 +1,60 @@
+// Element formats named by the caller (PCM_DT_*), independent of the 16-bit format this build's contractions use: the alignment losses and the
+// gradient-norm kernels take 32-bit, bfloat16 and IEEE-half tensors in every build of the library.
+#pragma once
+#include "pcm_common.h"
+
+struct DtF32 {
+  typedef float raw;
+  static constexpr int VEC = 4;      // elements of a 16-byte access
+  static __device__ __forceinline__ float ld(raw r) { return r; }
+  static __device__ __forceinline__ raw st(float f) { return f; }
+};
+struct DtBf16 {
+  typedef unsigned short raw;
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float ld(raw r) { return __uint_as_float(((unsigned)r) << 16); }
+  static __device__ __forceinline__ raw st(float f) {        // round to nearest even, NaN kept quiet
+#ifdef PCM_HOST_EMU
+    unsigned u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (raw)((u >> 16) | 0x40);
+    return (raw)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+#else
+    return __builtin_bit_cast(raw, (__bf16)f);
+#endif
+  }
+};
+struct DtF16 {
+  typedef unsigned short raw;
+  static constexpr int VEC = 8;
+#ifdef PCM_HOST_EMU
+  static __device__ __forceinline__ float ld(raw r) { return pcm_emu::half_to_float(r); }
+  static __device__ __forceinline__ raw st(float f) { return pcm_emu::float_to_half(f); }
+#else
+  static __device__ __forceinline__ float ld(raw r) { return (float)__builtin_bit_cast(_Float16, r); }
+  static __device__ __forceinline__ raw st(float f) { return __builtin_bit_cast(raw, (_Float16)f); }
+#endif
+};
+// f(Dt{}) for the format a PCM_DT_* code names (checked by the caller)
+template <typename F>
+static inline void pcm_with_dtype(int dt, F&& f) {
+  if (dt == PCM_DT_F32) f(DtF32{});
+  else if (dt == PCM_DT_BF16) f(DtBf16{});
+  else f(DtF16{});
+}
+static inline bool pcm_dt_ok(int dt) { return dt == PCM_DT_F32 || dt == PCM_DT_BF16 || dt == PCM_DT_F16; }
+static inline size_t pcm_dt_size(int dt) { return dt == PCM_DT_F32 ? 4 : 2; }
+
+// sum over a workgroup of NT threads in a fixed order (wave tree, then the wave sums in wave order), returned to every thread.  `red` holds one
+// value per wave; the barriers at both ends let one buffer serve several sums.
+template <int NT, typename V>
+__device__ __forceinline__ V pcm_block_sum(V v, V* red) {
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if constexpr (NT == 64) return v;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  V t = red[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; w++) t += red[w];
+  return t;
+}

@@ -23,6 +23,11 @@ ACT_NONE, ACT_SILU, ACT_LEAKY, ACT_GEGLU = 0, 1, 2, 3
 SEG_PLAIN, SEG_CONV3X3 = 0, 1
 SRC_DIRECT, SRC_UPSAMPLE2, SRC_ZEROINS2 = 0, 1, 2
 
+DT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PCM_DT_*: element formats named per call (alignment operators)
+PAIR_KINDS = {"sigmoid": 0, "hinge": 1, "square": 2}
+POLICY_REDUCE = {"token": 0, "row": 1, "sum": 2}
+GRAD_CHUNK = 16384          # PCM_GRAD_CHUNK
+
 vp = C.c_void_p
 
 
@@ -55,6 +60,27 @@ class PackDesc(C.Structure):
 
 
 i32, i64, f32 = C.c_int, C.c_long, C.c_float
+
+
+class DenoisePreferenceArgs(C.Structure):
+    _fields_ = [(k, vp) for k in ("pred", "ref", "target", "weight", "dpred", "loss", "log_ratio", "workspace")] + [
+        ("workspace_bytes", C.c_size_t), ("pairs", i64), ("n", i64), ("beta", C.c_double), ("label_smoothing", C.c_double), ("grad_scale", C.c_double),
+        ("dtype", i32), ("kind", i32), ("mean_reduce", i32)]
+
+
+class PreferenceArgs(C.Structure):
+    _fields_ = [(k, vp) for k in ("logp", "ref_logp", "mask", "lengths", "dlogp", "loss", "log_ratio", "workspace")] + [
+        ("workspace_bytes", C.c_size_t)] + [(k, i64) for k in ("pairs", "cols", "ld_logp", "ld_ref", "ld_mask", "ld_dlogp")] + [
+        ("beta", C.c_double), ("label_smoothing", C.c_double), ("grad_scale", C.c_double)] + [
+        (k, i32) for k in ("dtype", "kind", "mean_reduce", "lengths_i64")]
+
+
+class PolicyArgs(C.Structure):
+    _fields_ = [(k, vp) for k in ("logp", "old_logp", "ref_logp", "advantages", "mask", "lengths", "dlogp", "loss", "stats", "workspace")] + [
+        ("workspace_bytes", C.c_size_t)] + [(k, i64) for k in ("rows", "cols", "ld_logp", "ld_old", "ld_ref", "ld_adv", "ld_mask", "ld_dlogp")] + [
+        (k, C.c_double) for k in ("clip_low", "clip_high", "kl_coef", "grad_scale")] + [(k, i32) for k in ("dtype", "reduce", "adv_per_row", "lengths_i64")]
+
+
 _PROTOS = {
     "pcm_gemm_bf16": [C.POINTER(GemmSeg), i32, C.POINTER(GemmEpi), vp],
     "pcm_lora_wgrad_bf16": [C.POINTER(WgradArgs), vp],
@@ -138,6 +164,13 @@ _PROTOS = {
     "pcm_pack_segmented": [vp, vp, vp, vp, i32, i32, vp],
     "pcm_cast_f32_bf16": [vp, vp, i64, vp],
     "pcm_cast_bf16_f32": [vp, vp, i64, vp],
+    "pcm_transition_logprob": [vp, vp, vp, i32, i32, vp, i64, i64, vp, C.c_size_t, vp],
+    "pcm_transition_logprob_bwd": [vp, vp, vp, vp, i32, i32, vp, i64, i64, vp],
+    "pcm_denoise_preference_loss": [C.POINTER(DenoisePreferenceArgs), vp],
+    "pcm_preference_loss": [C.POINTER(PreferenceArgs), vp],
+    "pcm_policy_loss": [C.POINTER(PolicyArgs), vp],
+    "pcm_grad_norm": [vp, vp, i32, vp, vp, vp, C.c_size_t, vp],
+    "pcm_grad_clip": [vp, vp, i32, C.c_double, vp, vp, vp, C.c_size_t, vp],
 }
 
 
@@ -194,7 +227,10 @@ class Lib:
         self.dll.pcm_colsum_workspace_bytes.restype = C.c_size_t
         self.dll.pcm_colsum_workspace_bytes.argtypes = [C.c_int] * 3
         for name, argt in (("pcm_rowdot_bwd_workspace_bytes", [C.c_long, C.c_int]), ("pcm_groupnorm_param_grad_workspace_bytes", [C.c_int] * 4),
-                           ("pcm_mod_grad_workspace_bytes", [C.c_int] * 3)):        # abi 5
+                           ("pcm_mod_grad_workspace_bytes", [C.c_int] * 3),        # abi 5
+                           ("pcm_transition_logprob_workspace_bytes", [C.c_long] * 2), ("pcm_denoise_preference_loss_workspace_bytes", [C.c_long] * 2),
+                           ("pcm_preference_loss_workspace_bytes", [C.c_long] * 2), ("pcm_policy_loss_workspace_bytes", [C.c_long] * 2),
+                           ("pcm_grad_norm_workspace_bytes", [C.c_int])):        # abi 6
             f = getattr(self.dll, name, None)
             if f is not None:
                 f.restype, f.argtypes = C.c_size_t, argt

@@ -3,6 +3,7 @@ All activations are channels-last bf16 ``[B, H*W, C]`` / ``[M, C]`` torch tensor
 device-memory handles."""
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import capi
@@ -777,6 +778,320 @@ def sampler_ddim_step(eps_c, eps_u, x, alpha_t, alpha_prev, guidance):
     capi.lib().call("pcm_sampler_ddim_step", ptr(eps_c), ptr(eps_u), ptr(x), float(alpha_t), float(alpha_prev), float(guidance), ptr(out),
                     x.numel(), _stream())
     return out
+
+
+# ---- alignment of the distilled student: preference losses, clipped policy loss, transition log-probability, gradient norm and clipping ----
+# Loss and gradient come from one call, as in consistency_loss / hinge_loss.  Inputs are float32, bfloat16 or float16 (whatever the library's own
+# 16-bit format is), all of one call in the same format; losses, log ratios and statistics are float32.  Nothing synchronises; every call may be
+# captured in a hipGraph.  Sums run in a fixed order: results are bitwise the same run to run, with or without set_deterministic.
+def _one_place(name, **tensors):
+    """the one device of a call's tensors (Nones skipped)"""
+    dev = None
+    for k, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: {k} must be a tensor, got {type(t).__name__}")
+        if dev is None:
+            dev = t.device
+            if dev.type != "cuda" and torch.cuda.is_available():      # (CPU tensors are the host emulator's, where there is no GPU)
+                raise ValueError(f"{name}: {k} is on {dev}, not on the GPU")
+        elif t.device != dev:
+            raise ValueError(f"{name}: {k} is on {t.device}, the others on {dev}")
+    return dev
+
+
+def _one_format(name, **tensors):
+    """the PCM_DT_* code of a call's tensors, which must agree (Nones skipped)"""
+    first = None
+    for k, t in tensors.items():
+        if t is None:
+            continue
+        if first is None:
+            first = t.dtype
+            if first not in capi.DT_CODES:
+                raise TypeError(f"{name}: {k} must be float32, bfloat16 or float16, got {first}")
+        elif t.dtype != first:
+            raise TypeError(f"{name}: {k} is {t.dtype}, the others are {first}")
+    return capi.DT_CODES[first]
+
+
+def _row_stride(name, k, t, rows, cols):
+    """row stride of a [rows, cols] tensor with unit inner stride (rows may be apart, but must not overlap)"""
+    if t.shape != (rows, cols):
+        raise ValueError(f"{name}: {k} must be [{rows}, {cols}], got {list(t.shape)}")
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: {k} must have unit stride along its last dimension")
+    if rows == 1:
+        return cols
+    if t.stride(0) < cols:
+        raise ValueError(f"{name}: rows of {k} overlap (stride {t.stride(0)} < {cols})")
+    return t.stride(0)
+
+
+def _places(name, mask, lengths, rows, cols):
+    """checks of the optional mask [rows, cols] (bool / uint8) and lengths [rows] (int32 / int64) -> (mask row stride, lengths are int64)"""
+    ld = 0
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise TypeError(f"{name}: mask must be bool or uint8, got {mask.dtype}")
+        ld = _row_stride(name, "mask", mask, rows, cols)
+    if lengths is not None:
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{name}: lengths must be int32 or int64, got {lengths.dtype}")
+        if lengths.shape != (rows,) or not lengths.is_contiguous():
+            raise ValueError(f"{name}: lengths must be a contiguous [{rows}] tensor")
+    return ld, int(lengths is not None and lengths.dtype == torch.int64)
+
+
+def _choice(name, what, value, table):
+    if value not in table:
+        raise ValueError(f"{name}: {what} must be one of {sorted(table)}, got {value!r}")
+    return table[value]
+
+
+def _call_on(dev, name, *args):
+    """the call on ``dev``'s current stream, whichever device is the current one"""
+    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            capi.lib().call(name, *args, _stream())
+        return
+    capi.lib().call(name, *args, _stream())
+
+
+def _scratch(dev, nbytes):
+    return torch.empty(nbytes // 8, dtype=torch.float64, device=dev)
+
+
+def _transition_args(name, x, mean, std, **more):
+    dev = _one_place(name, x=x, mean=mean, std=std, **more)
+    dt = _one_format(name, x=x, mean=mean)
+    if x.dim() < 1 or x.shape != mean.shape or x.numel() == 0:
+        raise ValueError(f"{name}: x and mean must be non-empty and of one shape, got {list(x.shape)} and {list(mean.shape)}")
+    rows = x.shape[0]
+    for k, t in (("std", std),) + tuple(more.items()):
+        if t.shape != (rows,) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name}: {k} must be a contiguous float32 [{rows}] tensor")
+    if not (x.is_contiguous() and mean.is_contiguous()):
+        raise ValueError(f"{name}: x and mean must be contiguous")
+    return dev, dt, rows, x.numel() // rows
+
+
+def transition_logprob(x, mean, std, reduce="mean"):
+    """log-probability of a noisy sampler transition: x [B, ...] drawn from N(mean, std^2) with one std > 0 per sample (fp32 [B]) -> fp32 [B].
+    ``reduce`` "mean" divides by the elements of a sample, which keeps the difference of two log-probabilities (the policy ratio) well inside
+    fp32; "sum" is the density's logarithm itself."""
+    m = _choice("transition_logprob", "reduce", reduce, {"mean": 1, "sum": 0})
+    dev, dt, rows, n = _transition_args("transition_logprob", x, mean, std)
+    out = torch.empty(rows, dtype=torch.float32, device=dev)
+    nb = capi.lib().dll.pcm_transition_logprob_workspace_bytes(rows, n)
+    ws = _scratch(dev, nb)
+    _call_on(dev, "pcm_transition_logprob", ptr(x), ptr(mean), ptr(std), dt, m, ptr(out), rows, n, ptr(ws), nb)
+    return out
+
+
+def transition_logprob_bwd(x, mean, std, dlogp, reduce="mean"):
+    """gradient of transition_logprob by ``mean`` (same shape and format) from dlogp fp32 [B]"""
+    m = _choice("transition_logprob_bwd", "reduce", reduce, {"mean": 1, "sum": 0})
+    dev, dt, rows, n = _transition_args("transition_logprob_bwd", x, mean, std, dlogp=dlogp)
+    dmean = torch.empty_like(mean)
+    _call_on(dev, "pcm_transition_logprob_bwd", ptr(x), ptr(mean), ptr(std), ptr(dlogp), dt, m, ptr(dmean), rows, n)
+    return dmean
+
+
+def denoise_preference_loss(pred, ref_pred, target, weight=None, beta=2000.0, kind="sigmoid", label_smoothing=0.0, reduce="mean", grad_scale=1.0,
+                            want_grad=True):
+    """Preference loss of a denoiser: pred, ref_pred, target [2P, ...] are the student's and the frozen reference's predictions and what both should
+    have predicted; samples 0..P-1 are the preferred side of the pairs, P..2P-1 the rejected side.  Log ratio of a sample = -weight * (its squared
+    error - the reference's), squared errors averaged (``reduce`` "mean") or summed; weight fp32 [2P].  ``kind``: "sigmoid" (with label smoothing),
+    "hinge" or "square" (include/pcm_hip.h).  -> (loss [1], d(grad_scale * loss)/d pred, log ratios [2P])"""
+    name = "denoise_preference_loss"
+    m, kd = _choice(name, "reduce", reduce, {"mean": 1, "sum": 0}), _choice(name, "kind", kind, capi.PAIR_KINDS)
+    dev = _one_place(name, pred=pred, ref_pred=ref_pred, target=target, weight=weight)
+    dt = _one_format(name, pred=pred, ref_pred=ref_pred, target=target)
+    if pred.dim() < 1 or pred.shape[0] % 2 or pred.numel() == 0:
+        raise ValueError(f"{name}: pred must hold 2P > 0 samples, preferred then rejected, got {list(pred.shape)}")
+    for k, t in (("ref_pred", ref_pred), ("target", target)):
+        if t.shape != pred.shape:
+            raise ValueError(f"{name}: {k} must be {list(pred.shape)}, got {list(t.shape)}")
+    if not (pred.is_contiguous() and ref_pred.is_contiguous() and target.is_contiguous()):
+        raise ValueError(f"{name}: pred, ref_pred and target must be contiguous")
+    rows = pred.shape[0]
+    if weight is not None and (weight.shape != (rows,) or weight.dtype != torch.float32 or not weight.is_contiguous()):
+        raise ValueError(f"{name}: weight must be a contiguous float32 [{rows}] tensor")
+    n = pred.numel() // rows
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    ratio = torch.empty(rows, dtype=torch.float32, device=dev)
+    dpred = torch.empty_like(pred) if want_grad else None
+    nb = capi.lib().dll.pcm_denoise_preference_loss_workspace_bytes(rows // 2, n)
+    ws = _scratch(dev, nb)
+    a = capi.DenoisePreferenceArgs(ptr(pred), ptr(ref_pred), ptr(target), ptr(weight), ptr(dpred), ptr(loss), ptr(ratio), ptr(ws), nb, rows // 2, n,
+                                   beta, label_smoothing, grad_scale, dt, kd, m)
+    _call_on(dev, "pcm_denoise_preference_loss", C.byref(a))
+    return loss, dpred, ratio
+
+
+def preference_loss(logp, ref_logp, mask=None, lengths=None, beta=0.1, kind="sigmoid", label_smoothing=0.0, reduce="sum", grad_scale=1.0, want_grad=True):
+    """Preference loss from log-probabilities of tokens or sampler steps: logp, ref_logp [2P, T] of the policy and the frozen reference (rows may be
+    strided), rows 0..P-1 preferred, P..2P-1 rejected.  A place counts where ``mask`` (bool / uint8 [2P, T]) is set and before ``lengths`` (int32 /
+    int64 [2P]); what stands elsewhere is not used.  Log ratio of a row = sum (``reduce`` "mean": mean) of logp - ref_logp over its places, 0 if
+    it has none.  ``kind`` as in denoise_preference_loss.  -> (loss [1], d(grad_scale * loss)/d logp [2P, T], log ratios [2P])"""
+    name = "preference_loss"
+    m, kd = _choice(name, "reduce", reduce, {"mean": 1, "sum": 0}), _choice(name, "kind", kind, capi.PAIR_KINDS)
+    dev = _one_place(name, logp=logp, ref_logp=ref_logp, mask=mask, lengths=lengths)
+    dt = _one_format(name, logp=logp, ref_logp=ref_logp)
+    if logp.dim() != 2 or logp.shape[0] % 2 or logp.numel() == 0:
+        raise ValueError(f"{name}: logp must be [2P, T], preferred then rejected rows, got {list(logp.shape)}")
+    rows, cols = logp.shape
+    ldl, ldr = _row_stride(name, "logp", logp, rows, cols), _row_stride(name, "ref_logp", ref_logp, rows, cols)
+    ldm, l64 = _places(name, mask, lengths, rows, cols)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    ratio = torch.empty(rows, dtype=torch.float32, device=dev)
+    dlogp = torch.empty(rows, cols, dtype=logp.dtype, device=dev) if want_grad else None
+    nb = capi.lib().dll.pcm_preference_loss_workspace_bytes(rows // 2, cols)
+    ws = _scratch(dev, nb)
+    a = capi.PreferenceArgs(ptr(logp), ptr(ref_logp), ptr(mask), ptr(lengths), ptr(dlogp), ptr(loss), ptr(ratio), ptr(ws), nb, rows // 2, cols,
+                            ldl, ldr, ldm, cols, beta, label_smoothing, grad_scale, dt, kd, m, l64)
+    _call_on(dev, "pcm_preference_loss", C.byref(a))
+    return loss, dlogp, ratio
+
+
+def policy_loss(logp, advantages, old_logp=None, ref_logp=None, mask=None, lengths=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduce="token",
+                grad_scale=1.0, want_grad=True):
+    """Clipped policy loss with a KL term over log-probabilities [N, T] of tokens or sampler steps (rows may be strided):
+    -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(d) - d - 1), r = exp(logp - old_logp), d = ref_logp - logp.  ``old_logp`` None:
+    the policy itself.  advantages fp32 [N] or [N, T]; ``mask`` / ``lengths`` as in preference_loss.  ``reduce``: "token" (mean over all places),
+    "row" (mean over the N rows of each row's mean) or "sum".
+    -> (loss [1], d(grad_scale * loss)/d logp [N, T], stats [4] = objective, KL, share of places held by the clip, places)"""
+    name = "policy_loss"
+    rd = _choice(name, "reduce", reduce, capi.POLICY_REDUCE)
+    dev = _one_place(name, logp=logp, advantages=advantages, old_logp=old_logp, ref_logp=ref_logp, mask=mask, lengths=lengths)
+    dt = _one_format(name, logp=logp, old_logp=old_logp, ref_logp=ref_logp)
+    if logp.dim() != 2 or logp.numel() == 0:
+        raise ValueError(f"{name}: logp must be a non-empty [N, T] tensor, got {list(logp.shape)}")
+    if kl_coef != 0.0 and ref_logp is None:
+        raise ValueError(f"{name}: a KL term needs ref_logp")
+    rows, cols = logp.shape
+    if advantages.dtype != torch.float32:
+        raise TypeError(f"{name}: advantages must be float32, got {advantages.dtype}")
+    per_row = advantages.dim() == 1
+    if per_row and (advantages.shape != (rows,) or not advantages.is_contiguous()):
+        raise ValueError(f"{name}: advantages must be a contiguous [{rows}] or a [{rows}, {cols}] tensor, got {list(advantages.shape)}")
+    ldl = _row_stride(name, "logp", logp, rows, cols)
+    ldo = _row_stride(name, "old_logp", old_logp, rows, cols) if old_logp is not None else 0
+    ldr = _row_stride(name, "ref_logp", ref_logp, rows, cols) if ref_logp is not None else 0
+    lda = 0 if per_row else _row_stride(name, "advantages", advantages, rows, cols)
+    ldm, l64 = _places(name, mask, lengths, rows, cols)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    stats = torch.empty(4, dtype=torch.float32, device=dev)
+    dlogp = torch.empty(rows, cols, dtype=logp.dtype, device=dev) if want_grad else None
+    nb = capi.lib().dll.pcm_policy_loss_workspace_bytes(rows, cols)
+    ws = _scratch(dev, nb)
+    a = capi.PolicyArgs(ptr(logp), ptr(old_logp), ptr(ref_logp), ptr(advantages), ptr(mask), ptr(lengths), ptr(dlogp), ptr(loss), ptr(stats), ptr(ws), nb,
+                        rows, cols, ldl, ldo, ldr, lda, ldm, cols, clip_low, clip_high, kl_coef, grad_scale, dt, rd, int(per_row), l64)
+    _call_on(dev, "pcm_policy_loss", C.byref(a))
+    return loss, dlogp, stats
+
+
+def _dense_order(t):
+    """the dimensions of ``t`` from the fastest to the slowest if its elements fill one gapless range of memory, else None"""
+    dims = sorted((d for d in range(t.dim()) if t.shape[d] > 1), key=t.stride)
+    step = 1
+    for d in dims:
+        if t.stride(d) != step:
+            return None
+        step *= t.shape[d]
+    return dims
+
+
+class GradSet:
+    """The gradients of many parameters as one set: their global norm and their clipping in two launches, whatever their number, sizes and formats
+    (float32 / bfloat16 / float16 side by side; empty ones are skipped).  The addresses are taken here, once: build the set anew when gradients are
+    reallocated.  A captured call keeps using them, so the set has to outlive the graph.
+
+    ``out``: tensors that receive the clipped gradients (same shapes and element order, any of the formats; e.g. slices of a flat buffer); by
+    default the gradients are clipped in place.  Each tensor has to fill its memory without gaps, and no output may overlap another one or a
+    gradient other than its own."""
+
+    def __init__(self, grads, out=None):
+        grads = list(grads)
+        dsts = grads if out is None else list(out)
+        if len(grads) != len(dsts):
+            raise ValueError(f"GradSet: {len(grads)} gradients but {len(dsts)} outputs")
+        if not grads:
+            raise ValueError("GradSet: no gradients")
+        if not all(isinstance(t, torch.Tensor) for t in grads + dsts):
+            raise TypeError("GradSet: gradients and outputs must be tensors")
+        self.device = _one_place("GradSet", **{f"tensor {i}": t for i, t in enumerate(grads + (dsts if out is not None else []))})
+        spans, rows = [], []
+        for i, (g, o) in enumerate(zip(grads, dsts)):
+            for t in (g, o):
+                if t.dtype not in capi.DT_CODES:
+                    raise TypeError(f"GradSet: tensor {i} must be float32, bfloat16 or float16, got {t.dtype}")
+            if g.shape != o.shape:
+                raise ValueError(f"GradSet: output {i} must be {list(g.shape)}, got {list(o.shape)}")
+            if g.numel() == 0:
+                continue
+            order = _dense_order(g)
+            if order is None or _dense_order(o) != order:
+                raise ValueError(f"GradSet: gradient {i} and its output must each fill their memory without gaps, in the same element order")
+            s0, d0 = g.data_ptr(), o.data_ptr()
+            s1, d1 = s0 + g.numel() * g.element_size(), d0 + o.numel() * o.element_size()
+            own = s0 == d0 and g.dtype == o.dtype
+            spans.append((d0, d1, True))
+            if not own:
+                spans.append((s0, s1, False))
+            rows.append((s0, d0, g.numel(), capi.DT_CODES[g.dtype], capi.DT_CODES[o.dtype]))
+        end_any = end_out = 0
+        for a, b, is_out in sorted(spans):
+            if a < (end_any if is_out else end_out):
+                raise ValueError("GradSet: an output overlaps another output or a gradient that is not its own")
+            end_any = max(end_any, b)
+            end_out = max(end_out, b) if is_out else end_out
+        self._keep = (grads, dsts)
+        desc = np.array(rows, dtype=[("src", "<u8"), ("dst", "<u8"), ("n", "<i8"), ("sdt", "<i4"), ("ddt", "<i4")])
+        per = (desc["n"] + capi.GRAD_CHUNK - 1) // capi.GRAD_CHUNK
+        self.chunks = int(per.sum())
+        if self.chunks >= 2 ** 31:
+            raise ValueError("GradSet: too many elements")
+        tensor = np.repeat(np.arange(len(rows)), per)
+        first = np.repeat(np.cumsum(per) - per, per)
+        chunk = np.stack([(np.arange(self.chunks) - first) * capi.GRAD_CHUNK, tensor], axis=1).astype("<i8")
+        self._cut = desc.nbytes
+        table = np.concatenate([np.frombuffer(desc.tobytes(), np.uint8), np.frombuffer(chunk.tobytes(), np.uint8)])
+        self._table = torch.from_numpy(table.copy()).to(self.device)
+        self._stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
+
+    def _run(self, name, sumsq, *more):
+        dev = self.device
+        if sumsq is None:
+            sumsq = torch.empty(1, dtype=torch.float64, device=dev)
+        elif sumsq.dtype != torch.float64 or sumsq.numel() != 1 or sumsq.device != dev:
+            raise ValueError(f"GradSet: sumsq must be one float64 on {dev}")
+        if self.chunks == 0:
+            sumsq.zero_()
+            return torch.zeros(1, dtype=torch.float32, device=dev)
+        norm = torch.empty(1, dtype=torch.float32, device=dev)
+        nb = capi.lib().dll.pcm_grad_norm_workspace_bytes(self.chunks)
+        ws = _scratch(dev, nb)
+        base = self._table.data_ptr()
+        _call_on(dev, name, base, base + self._cut, self.chunks, *more, ptr(norm), ptr(sumsq), ptr(ws), nb)
+        if self._stream is not None and not torch.cuda.is_current_stream_capturing():
+            now = torch.cuda.current_stream(dev)
+            if now != self._stream:
+                self._table.record_stream(now)        # the tables were allocated on another stream: not reused before this call is through
+        return norm
+
+    def norm(self, sumsq=None):
+        """sqrt of the sum of all squares, fp32 [1]; ``sumsq`` (fp64 [1], optional) receives the sum itself (what adamw_clip_step takes as gradsq)"""
+        return self._run("pcm_grad_norm", sumsq)
+
+    def clip(self, max_norm, sumsq=None):
+        """scales the gradients by min(1, max_norm / (norm + 1e-6)) -- in place, or into ``out`` -- and returns the norm before clipping, fp32 [1].  A
+        norm that is not finite reaches the gradients as the formula has it (nan, or 0 and nan): check the returned norm."""
+        if not max_norm > 0:
+            raise ValueError(f"GradSet.clip: max_norm must be positive, got {max_norm}")
+        return self._run("pcm_grad_clip", sumsq, float(max_norm))
 
 
 def __getattr__(name):
