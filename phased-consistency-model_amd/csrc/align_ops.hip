@@ -9,32 +9,97 @@
 #define AL_LOOP(i, n) for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < (n); i += (long)gridDim.x * blockDim.x)
 static inline int al_blocks(long n) { long b = (n + 255) / 256; return (int)(b > PCM_GRID_CAP(2048) ? PCM_GRID_CAP(2048) : (b < 1 ? 1 : b)); }
 
+// ---- work of one team (a wave or a workgroup of NT threads) on elements [i0, i1) of a row, U groups of 16 bytes per thread in flight ----
+// f(idx, left): the group of VEC elements at idx, `left` of them inside the range (>= VEC: all)
+template <typename Dt, int NT, int U, typename Load, typename Use>
+__device__ __forceinline__ void al_groups(long i0, long i1, int tid, Load&& load, Use&& use) {
+  constexpr long STEP = (long)NT * Dt::VEC;
+  long i = i0 + (long)tid * Dt::VEC;
+  for (; i + (U - 1) * STEP + Dt::VEC <= i1; i += U * STEP) {
+#pragma unroll
+    for (int u = 0; u < U; u++) load(u, i + u * STEP, (long)Dt::VEC);
+#pragma unroll
+    for (int u = 0; u < U; u++) use(u, i + u * STEP, (long)Dt::VEC);
+  }
+  for (; i < i1; i += STEP) { load(0, i, i1 - i); use(0, i, i1 - i); }
+}
+// how a launch cuts rows of n elements: teams of 64 (four rows to a workgroup) for short rows, else `chunks` workgroups of 256 per row, so that some
+// 2048 workgroups (8 per CU) share the work; at most 64 chunks, whose partial sums one wave adds up with one load per lane.
+struct RowCut { int team, chunks; long len; };
+static RowCut row_cut(long rows, long n, int vec) {
+  RowCut c = {256, 1, n};
+  if (n <= 1024) { c.team = 64; return c; }
+  const long unit = 256L * vec, most = (n + unit - 1) / unit, want = 2048 / rows;
+  long k = want < 1 ? 1 : (want < most ? want : most);
+  if (k > 64) k = 64;
+  c.len = ((n + k - 1) / k + unit - 1) / unit * unit;
+  c.chunks = (int)((n + c.len - 1) / c.len);
+  return c;
+}
+static inline unsigned row_cut_blocks(const RowCut& c, long rows) { return (unsigned)(c.team == 64 ? (rows + 3) / 4 : rows * c.chunks); }
+// (row, chunk, thread of the team) of a thread; false: a team past the last row
+template <int TEAM>
+__device__ __forceinline__ bool row_cut_place(long block, long rows, int chunks, long* row, int* chunk, int* tid) {
+  if (TEAM == 64) { *row = block * 4 + (threadIdx.x >> 6); *chunk = 0; *tid = threadIdx.x & 63; return *row < rows; }
+  *row = block / chunks; *chunk = (int)(block - *row * chunks); *tid = threadIdx.x;
+  return true;
+}
+
 // ---- log-probability of x ~ N(mean, std^2) per row:  -1/2 sum ((x - mean) / std)^2 - n log std - n/2 log 2 pi   (/ n) ----
 #define LOG_2PI 1.8378770664093454836
-template <typename Dt>
-__global__ __launch_bounds__(256) void transition_fwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std, float* logp,
-                                                             long n, int mean_reduce) {
+__device__ __forceinline__ float transition_value(double acc, double s, long n, int mean_reduce) {
+  const double per = -0.5 * acc / (s * s * (double)n) - log(s) - 0.5 * LOG_2PI;
+  return (float)(mean_reduce ? per : per * (double)n);
+}
+template <typename Dt, int TEAM>
+__global__ __launch_bounds__(256) void transition_fwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std, float* logp, double* part,
+                                                             long rows, long n, int chunks, long len, int mean_reduce) {
   __shared__ double red[4];
-  const long row = blockIdx.x;
-  x += row * n; mean += row * n;
+  long row; int chunk, tid;
+  if (!row_cut_place<TEAM>(blockIdx.x, rows, chunks, &row, &chunk, &tid)) return;
+  const long i0 = chunk * len, i1 = i0 + len < n ? i0 + len : n;
+  const typename Dt::raw *xr = x + row * n, *mr = mean + row * n;
+  float a[4][Dt::VEC], b[4][Dt::VEC];
   double acc = 0.0;
-  for (long i = threadIdx.x; i < n; i += 256) { const float d = Dt::ld(x[i]) - Dt::ld(mean[i]); acc += (double)(d * d); }
-  acc = pcm_block_sum<256>(acc, red);
-  if (threadIdx.x == 0) {
-    const double s = (double)std[row];
-    const double per = -0.5 * acc / (s * s * (double)n) - log(s) - 0.5 * LOG_2PI;
-    logp[row] = (float)(mean_reduce ? per : per * (double)n);
+  al_groups<Dt, TEAM, 4>(i0, i1, tid,
+    [&](int u, long i, long left) { pcm_ld_group<Dt>(xr + i, left, a[u]); pcm_ld_group<Dt>(mr + i, left, b[u]); },
+    [&](int u, long i, long left) {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < Dt::VEC; j++) { const float d = a[u][j] - b[u][j]; t += d * d; }
+      acc += (double)t;
+    });
+  acc = pcm_block_sum<TEAM>(acc, red);
+  if (tid == 0) {
+    if (chunks == 1) logp[row] = transition_value(acc, (double)std[row], n, mean_reduce);
+    else part[row * chunks + chunk] = acc;
   }
 }
-template <typename Dt>
+__global__ __launch_bounds__(256) void transition_finish_kernel(const double* part, const float* std, float* logp, long rows, long n, int chunks, int mean_reduce) {
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const double acc = pcm_lane_sum(lane < chunks ? part[row * chunks + lane] : 0.0);
+  if (lane == 0) logp[row] = transition_value(acc, (double)std[row], n, mean_reduce);
+}
+template <typename Dt, int TEAM>
 __global__ __launch_bounds__(256) void transition_bwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std,
-                                                             const float* dlogp, typename Dt::raw* dmean, long rows, long n, int mean_reduce) {
-  AL_LOOP(i, rows * n) {
-    const long row = i / n;
-    const double s = (double)std[row];
-    const float f = (float)((double)dlogp[row] / (s * s * (mean_reduce ? (double)n : 1.0)));
-    dmean[i] = Dt::st((Dt::ld(x[i]) - Dt::ld(mean[i])) * f);
-  }
+                                                             const float* dlogp, typename Dt::raw* dmean, long rows, long n, int chunks, long len, int mean_reduce) {
+  long row; int chunk, tid;
+  if (!row_cut_place<TEAM>(blockIdx.x, rows, chunks, &row, &chunk, &tid)) return;
+  const long i0 = chunk * len, i1 = i0 + len < n ? i0 + len : n;
+  const typename Dt::raw *xr = x + row * n, *mr = mean + row * n;
+  typename Dt::raw* dr = dmean + row * n;
+  const double s = (double)std[row];
+  const float f = (float)((double)dlogp[row] / (s * s * (mean_reduce ? (double)n : 1.0)));
+  float a[4][Dt::VEC], b[4][Dt::VEC];
+  al_groups<Dt, TEAM, 4>(i0, i1, tid,
+    [&](int u, long i, long left) { pcm_ld_group<Dt>(xr + i, left, a[u]); pcm_ld_group<Dt>(mr + i, left, b[u]); },
+    [&](int u, long i, long left) {
+#pragma unroll
+      for (int j = 0; j < Dt::VEC; j++) a[u][j] = (a[u][j] - b[u][j]) * f;
+      pcm_st_group<Dt>(dr + i, left, a[u]);
+    });
 }
 
 // ---- preference losses.  rows [0, P) are the preferred side, [P, 2P) the rejected side; rho = log ratio of a row ----
@@ -56,43 +121,53 @@ __device__ __forceinline__ void pair_loss(const PairLoss p, double h, double* lo
     *slope = 2.0 * gap;
   }
 }
-__global__ __launch_bounds__(256) void pair_finish_kernel(const double* rho, PairLoss pl, long pairs, float* loss, float* log_ratio) {
-  __shared__ double red[4];
-  double acc = 0.0;
-  for (long p = threadIdx.x; p < pairs; p += 256) {
-    double l, s;
-    pair_loss(pl, rho[p] - rho[pairs + p], &l, &s);
-    acc += l;
-    log_ratio[p] = (float)rho[p];
-    log_ratio[pairs + p] = (float)rho[pairs + p];
+// A source of log ratios gives, for a range of a row: sums() -- what the thread adds to the row's sums; and grad() -- its part of the gradient, f being
+// the row's factor.  rho() and factor() turn a row's sums into its log ratio and into what multiplies the pair's slope in f.
+// Denoising errors: rho = -w k sum ((t - p)^2 - (t - r)^2);  d rho / d p = 2 w k (t - p)
+template <typename Dt_>
+struct DenoiseRows {
+  typedef Dt_ Dt;
+  typedef typename Dt::raw raw;
+  const raw *pred, *ref, *target;
+  const float* weight;
+  raw* dpred;
+  double k;
+  long n;
+  static constexpr int SUMS = 1;
+  template <int NT>
+  __device__ __forceinline__ void sums(long row, long i0, long i1, int tid, double (&acc)[SUMS]) const {
+    const long o = row * n;
+    float t[4][Dt::VEC], p[4][Dt::VEC], r[4][Dt::VEC];
+    double s = 0.0;
+    al_groups<Dt, NT, 4>(i0, i1, tid,
+      [&](int u, long i, long left) {
+        pcm_ld_group<Dt>(target + o + i, left, t[u]); pcm_ld_group<Dt>(pred + o + i, left, p[u]); pcm_ld_group<Dt>(ref + o + i, left, r[u]);
+      },
+      [&](int u, long i, long left) {
+        float e = 0.f;
+#pragma unroll
+        for (int j = 0; j < Dt::VEC; j++) { const float a = t[u][j] - p[u][j], b = t[u][j] - r[u][j]; e += a * a - b * b; }
+        s += (double)e;
+      });
+    acc[0] = s;
   }
-  acc = pcm_block_sum<256>(acc, red);
-  if (threadIdx.x == 0) loss[0] = (float)(acc / (double)pairs);
-}
-// rho of one row of denoising errors: -w k sum ((t - p)^2 - (t - r)^2)
-template <typename Dt>
-__global__ __launch_bounds__(256) void denoise_rho_kernel(const typename Dt::raw* pred, const typename Dt::raw* ref, const typename Dt::raw* target,
-                                                          const float* weight, double k, double* rho, long n) {
-  __shared__ double red[4];
-  const long row = blockIdx.x;
-  double acc = 0.0;
-  for (long i = row * n + threadIdx.x; i < (row + 1) * n; i += 256) {
-    const float t = Dt::ld(target[i]), a = t - Dt::ld(pred[i]), b = t - Dt::ld(ref[i]);
-    acc += (double)(a * a - b * b);
+  template <int NT>
+  __device__ __forceinline__ void grad(long row, long i0, long i1, int tid, float f) const {
+    const long o = row * n;
+    float t[4][Dt::VEC], p[4][Dt::VEC];
+    al_groups<Dt, NT, 4>(i0, i1, tid,
+      [&](int u, long i, long left) { pcm_ld_group<Dt>(target + o + i, left, t[u]); pcm_ld_group<Dt>(pred + o + i, left, p[u]); },
+      [&](int u, long i, long left) {
+#pragma unroll
+        for (int j = 0; j < Dt::VEC; j++) t[u][j] = (t[u][j] - p[u][j]) * f;
+        pcm_st_group<Dt>(dpred + o + i, left, t[u]);
+      });
   }
-  acc = pcm_block_sum<256>(acc, red);
-  if (threadIdx.x == 0) rho[row] = -acc * k * (weight ? (double)weight[row] : 1.0);
-}
-template <typename Dt>
-__global__ __launch_bounds__(256) void denoise_grad_kernel(const typename Dt::raw* pred, const typename Dt::raw* target, const float* weight, double k,
-                                                           const double* rho, PairLoss pl, double gscale, typename Dt::raw* dpred, long pairs, long n) {
-  const long row = blockIdx.x, p = row < pairs ? row : row - pairs;
-  double l, s;
-  pair_loss(pl, rho[p] - rho[pairs + p], &l, &s);
-  const float f = (float)((row < pairs ? 2.0 : -2.0) * s * k * gscale / (double)pairs * (weight ? (double)weight[row] : 1.0));
-  for (long i = row * n + threadIdx.x; i < (row + 1) * n; i += 256) dpred[i] = Dt::st((Dt::ld(target[i]) - Dt::ld(pred[i])) * f);
-}
-
+  __device__ __forceinline__ double scale(long row) const { return k * (weight ? (double)weight[row] : 1.0); }
+  __device__ __forceinline__ double rho(long row, const double (&s)[SUMS]) const { return -s[0] * scale(row); }
+  __device__ __forceinline__ double factor(long row, const double (&s)[SUMS]) const { return 2.0 * scale(row); }
+  bool wants_grad() const { return dpred != nullptr; }
+};
 // places that count: mask[row][col] != 0 (or no mask) and col < lengths[row] (or no lengths)
 struct Places {
   const unsigned char* mask; long ld_mask;
@@ -103,37 +178,151 @@ struct Places {
     const long v = i64 ? (long)((const int64_t*)lengths)[row] : (long)((const int32_t*)lengths)[row];
     return v < 0 ? 0 : (v > cols ? cols : v);
   }
+  // bit j: place c + j of the row counts, c + j < c + left and < len
+  template <int VEC>
+  __device__ __forceinline__ unsigned bits(long row, long c, long len) const {
+    const long left = len - c;
+    if (left <= 0) return 0u;
+    unsigned in = left >= VEC ? (1u << VEC) - 1u : (1u << left) - 1u;
+    if (mask) {
+      const unsigned char* m = mask + row * ld_mask + c;
+      unsigned got = 0u;
+      if (left >= VEC) {
+        typedef unsigned char mv __attribute__((ext_vector_type(VEC), aligned(1)));
+        const mv b = *(const mv*)m;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) got |= b[j] ? 1u << j : 0u;
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          if (j < left) got |= m[j] ? 1u << j : 0u;
+      }
+      in &= got;
+    }
+    return in;
+  }
 };
-template <typename Dt>
-__global__ __launch_bounds__(256) void preference_rho_kernel(const typename Dt::raw* logp, long ld_logp, const typename Dt::raw* ref, long ld_ref, Places pc,
-                                                             int mean_reduce, double* rho, double* share) {
+// log-probabilities: rho = sum (mean) over the places that count of logp - ref;  d rho / d logp = 1 (1 / count) there
+template <typename Dt_>
+struct TokenRows {
+  typedef Dt_ Dt;
+  typedef typename Dt::raw raw;
+  const raw* logp; long ld_logp;
+  const raw* ref; long ld_ref;
+  Places pc;
+  raw* dlogp; long ld_d;
+  int mean_reduce;
+  static constexpr int SUMS = 2;
+  template <int NT>
+  __device__ __forceinline__ void sums(long row, long i0, long i1, int tid, double (&acc)[SUMS]) const {
+    const raw *lr = logp + row * ld_logp, *rr = ref + row * ld_ref;
+    const long len = pc.len(row);
+    float a[2][Dt::VEC], b[2][Dt::VEC];
+    unsigned in[2];
+    double s = 0.0;
+    int cnt = 0;
+    al_groups<Dt, NT, 2>(i0, len < i1 ? len : i1, tid,
+      [&](int u, long i, long left) {
+        in[u] = pc.bits<Dt::VEC>(row, i, len);
+        pcm_ld_group<Dt>(lr + i, left, a[u]); pcm_ld_group<Dt>(rr + i, left, b[u]);
+      },
+      [&](int u, long i, long left) {
+        float e = 0.f;
+#pragma unroll
+        for (int j = 0; j < Dt::VEC; j++) { e += in[u] >> j & 1u ? a[u][j] - b[u][j] : 0.f; cnt += in[u] >> j & 1u; }
+        s += (double)e;
+      });
+    acc[0] = s; acc[1] = (double)cnt;
+  }
+  template <int NT>
+  __device__ __forceinline__ void grad(long row, long i0, long i1, int tid, float f) const {
+    const long len = pc.len(row);
+    unsigned in[2];
+    al_groups<Dt, NT, 2>(i0, i1, tid,
+      [&](int u, long i, long left) { in[u] = pc.bits<Dt::VEC>(row, i, len); },
+      [&](int u, long i, long left) {
+        float g[Dt::VEC];
+#pragma unroll
+        for (int j = 0; j < Dt::VEC; j++) g[j] = in[u] >> j & 1u ? f : 0.f;
+        pcm_st_group<Dt>(dlogp + row * ld_d + i, left, g);
+      });
+  }
+  __device__ __forceinline__ double share(const double (&s)[SUMS]) const { return mean_reduce ? 1.0 / fmax(s[1], 1.0) : 1.0; }
+  __device__ __forceinline__ double rho(long row, const double (&s)[SUMS]) const { return s[0] * share(s); }
+  __device__ __forceinline__ double factor(long row, const double (&s)[SUMS]) const { return share(s); }
+  bool wants_grad() const { return dlogp != nullptr; }
+};
+// Two launches: (1) partial sums of every (row, chunk); (2) the gradient, where each team adds up the partial sums of its pair again instead of
+// waiting for a launch that does it once -- at most 2 x 64 numbers out of L2 -- and the first workgroup forms the mean loss.
+template <typename R, int TEAM>
+__global__ __launch_bounds__(256) void pair_sums_kernel(R rows_, double* part, long rows, long n, int chunks, long len) {
   __shared__ double red[4];
-  __shared__ long redl[4];
-  const long row = blockIdx.x, len = pc.len(row);
-  double acc = 0.0;
-  long cnt = 0;
-  for (long c = threadIdx.x; c < len; c += 256) {
-    if (pc.mask && !pc.mask[row * pc.ld_mask + c]) continue;
-    acc += (double)(Dt::ld(logp[row * ld_logp + c]) - Dt::ld(ref[row * ld_ref + c]));
-    cnt++;
-  }
-  acc = pcm_block_sum<256>(acc, red);
-  cnt = pcm_block_sum<256>(cnt, redl);
-  if (threadIdx.x == 0) {
-    const double sh = mean_reduce ? 1.0 / (double)(cnt > 0 ? cnt : 1) : 1.0;
-    rho[row] = acc * sh;
-    share[row] = sh;
-  }
+  long row; int chunk, tid;
+  if (!row_cut_place<TEAM>(blockIdx.x, rows, chunks, &row, &chunk, &tid)) return;
+  const long i0 = chunk * len, i1 = i0 + len < n ? i0 + len : n;
+  double acc[R::SUMS];
+  rows_.template sums<TEAM>(row, i0, i1, tid, acc);
+#pragma unroll
+  for (int a = 0; a < R::SUMS; a++) acc[a] = pcm_block_sum<TEAM>(acc[a], red);
+  if (tid == 0)
+#pragma unroll
+    for (int a = 0; a < R::SUMS; a++) part[(row * chunks + chunk) * R::SUMS + a] = acc[a];
 }
-template <typename Dt>
-__global__ __launch_bounds__(256) void preference_grad_kernel(Places pc, const double* rho, const double* share, PairLoss pl, double gscale,
-                                                              typename Dt::raw* dlogp, long ld_d, long pairs) {
-  const long row = blockIdx.x, len = pc.len(row), p = row < pairs ? row : row - pairs;
-  double l, s;
-  pair_loss(pl, rho[p] - rho[pairs + p], &l, &s);
-  const float f = (float)((row < pairs ? 1.0 : -1.0) * s * share[row] * gscale / (double)pairs);
-  for (long c = threadIdx.x; c < pc.cols; c += 256)
-    dlogp[row * ld_d + c] = Dt::st(c < len && (!pc.mask || pc.mask[row * pc.ld_mask + c]) ? f : 0.f);
+template <typename R>
+__device__ __forceinline__ void pair_row_total(const double* part, long row, int chunks, int lane, double (&s)[R::SUMS]) {
+#pragma unroll
+  for (int a = 0; a < R::SUMS; a++) s[a] = pcm_lane_sum(lane < chunks ? part[(row * chunks + lane) * R::SUMS + a] : 0.0);
+}
+template <typename R, int TEAM>
+__global__ __launch_bounds__(256) void pair_grad_kernel(R rows_, const double* part, PairLoss pl, double gscale, float* loss, float* log_ratio, long pairs,
+                                                        long n, int chunks, long len) {
+  __shared__ double red[4];
+  if (blockIdx.x == 0) {
+    double acc = 0.0;
+    for (long p = threadIdx.x; p < pairs; p += 256) {
+      double rho[2], l, s;
+      for (int side = 0; side < 2; side++) {
+        const long row = p + side * pairs;
+        double t[R::SUMS];
+#pragma unroll
+        for (int a = 0; a < R::SUMS; a++) t[a] = 0.0;
+        for (int c = 0; c < chunks; c++)
+#pragma unroll
+          for (int a = 0; a < R::SUMS; a++) t[a] += part[(row * chunks + c) * R::SUMS + a];
+        rho[side] = rows_.rho(row, t);
+        log_ratio[row] = (float)rho[side];
+      }
+      pair_loss(pl, rho[0] - rho[1], &l, &s);
+      acc += l;
+    }
+    acc = pcm_block_sum<256>(acc, red);
+    if (threadIdx.x == 0) loss[0] = (float)(acc / (double)pairs);
+    return;
+  }
+  long row; int chunk, tid;
+  if (!row_cut_place<TEAM>(blockIdx.x - 1, 2 * pairs, chunks, &row, &chunk, &tid)) return;
+  const long i0 = chunk * len, i1 = i0 + len < n ? i0 + len : n, p = row < pairs ? row : row - pairs;
+  double up[R::SUMS], down[R::SUMS], l, s;
+  pair_row_total<R>(part, p, chunks, threadIdx.x & 63, up);
+  pair_row_total<R>(part, pairs + p, chunks, threadIdx.x & 63, down);
+  pair_loss(pl, rows_.rho(p, up) - rows_.rho(pairs + p, down), &l, &s);
+  const double f = (row < pairs ? s * rows_.factor(row, up) : -s * rows_.factor(row, down)) * gscale / (double)pairs;
+  rows_.template grad<TEAM>(row, i0, i1, tid, (float)f);
+}
+// bytes of the partial sums
+static size_t pair_ws_bytes(long rows, long n, int vec, int sums) { const RowCut c = row_cut(rows, n, vec); return (size_t)rows * c.chunks * sums * sizeof(double); }
+template <typename R>
+static void pair_launch(const R& r, double* part, const PairLoss& pl, double gscale, float* loss, float* log_ratio, long pairs, long n, void* stream) {
+  const long rows = 2 * pairs;
+  const RowCut c = row_cut(rows, n, R::Dt::VEC);
+  const unsigned nb = row_cut_blocks(c, rows), ng = r.wants_grad() ? nb + 1 : 1;
+  if (c.team == 64) {
+    PCM_LAUNCH((pair_sums_kernel<R, 64>), dim3(nb), dim3(256), 0, stream, r, part, rows, n, c.chunks, c.len);
+    PCM_LAUNCH((pair_grad_kernel<R, 64>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, loss, log_ratio, pairs, n, c.chunks, c.len);
+  } else {
+    PCM_LAUNCH((pair_sums_kernel<R, 256>), dim3(nb), dim3(256), 0, stream, r, part, rows, n, c.chunks, c.len);
+    PCM_LAUNCH((pair_grad_kernel<R, 256>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, loss, log_ratio, pairs, n, c.chunks, c.len);
+  }
 }
 
 // ---- clipped policy loss with a KL term ----
@@ -222,17 +411,30 @@ __global__ __launch_bounds__(256) void policy_finish_kernel(const double* part, 
 }
 
 // ---- entry points ----
-#define AL_MAX_ROWS 2147483647L
-extern "C" size_t pcm_transition_logprob_workspace_bytes(long rows, long n) { return rows > 0 && n > 0 ? 8 : 0; }
+#define AL_MAX_ROWS 16777216L       /* 64 chunks of a row at the most: a grid stays below 2^31 workgroups */
+extern "C" size_t pcm_transition_logprob_workspace_bytes(long rows, long n) {
+  if (rows <= 0 || n <= 0) return 0;
+  const RowCut c = row_cut(rows, n, 4);      // (the 16-bit formats cut into no more chunks than fp32)
+  return c.chunks > 1 ? (size_t)rows * c.chunks * sizeof(double) : 0;
+}
+#define TRANSITION_LAUNCH(kernel, ...)                                                                                       \
+  do {                                                                                                                       \
+    if (c.team == 64) PCM_LAUNCH((kernel<Dt, 64>), dim3(row_cut_blocks(c, rows)), dim3(256), 0, stream, __VA_ARGS__);        \
+    else PCM_LAUNCH((kernel<Dt, 256>), dim3(row_cut_blocks(c, rows)), dim3(256), 0, stream, __VA_ARGS__);                    \
+  } while (0)
 extern "C" int pcm_transition_logprob(const void* x, const void* mean, const float* std, int dtype, int mean_reduce, float* logp, long rows, long n,
                                       void* workspace, size_t workspace_bytes, void* stream) {
   PCM_CHECK(x && mean && std && logp && pcm_dt_ok(dtype) && rows > 0 && rows <= AL_MAX_ROWS && n > 0, PCM_EINVAL, "pcm_transition_logprob: null/empty or unknown format");
-  PCM_CHECK(workspace && ((uintptr_t)workspace % 8) == 0 && workspace_bytes >= pcm_transition_logprob_workspace_bytes(rows, n), PCM_EINVAL,
+  const size_t need = pcm_transition_logprob_workspace_bytes(rows, n);
+  PCM_CHECK(need == 0 || (workspace && ((uintptr_t)workspace % 8) == 0 && workspace_bytes >= need), PCM_EINVAL,
             "pcm_transition_logprob: workspace too small or not 8-byte aligned");
   pcm_with_dtype(dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    PCM_LAUNCH(transition_fwd_kernel<Dt>, dim3((unsigned)rows), dim3(256), 0, stream, (cp)x, (cp)mean, std, logp, n, mean_reduce);
+    const RowCut c = row_cut(rows, n, Dt::VEC);
+    TRANSITION_LAUNCH(transition_fwd_kernel, (cp)x, (cp)mean, std, logp, (double*)workspace, rows, n, c.chunks, c.len, mean_reduce);
+    if (c.chunks > 1)
+      PCM_LAUNCH(transition_finish_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, (const double*)workspace, std, logp, rows, n, c.chunks, mean_reduce);
   });
   return pcm_post_launch("pcm_transition_logprob");
 }
@@ -243,7 +445,8 @@ extern "C" int pcm_transition_logprob_bwd(const void* x, const void* mean, const
   pcm_with_dtype(dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    PCM_LAUNCH(transition_bwd_kernel<Dt>, dim3(al_blocks(rows * n)), dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, mean_reduce);
+    const RowCut c = row_cut(rows, n, Dt::VEC);
+    TRANSITION_LAUNCH(transition_bwd_kernel, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, c.chunks, c.len, mean_reduce);
   });
   return pcm_post_launch("pcm_transition_logprob_bwd");
 }
@@ -256,7 +459,7 @@ static int pair_args_ok(const char* who, int dtype, long pairs, double beta, int
   PCM_CHECK(eps >= 0.0 && eps < 0.5 && (eps == 0.0 || kind == PCM_PAIR_SIGMOID), PCM_EINVAL, "%s: label smoothing must be in [0, 0.5) and needs the sigmoid kind", who);
   return PCM_OK;
 }
-extern "C" size_t pcm_denoise_preference_loss_workspace_bytes(long pairs, long n) { return pairs > 0 && n > 0 ? 2 * (size_t)pairs * sizeof(double) : 0; }
+extern "C" size_t pcm_denoise_preference_loss_workspace_bytes(long pairs, long n) { return pairs > 0 && n > 0 ? pair_ws_bytes(2 * pairs, n, 4, DenoiseRows<DtF32>::SUMS) : 0; }
 extern "C" int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a, void* stream) {
   PCM_CHECK(a && a->pred && a->ref && a->target && a->loss && a->log_ratio && a->n > 0, PCM_EINVAL, "pcm_denoise_preference_loss: null/empty");
   const int rc = pair_args_ok("pcm_denoise_preference_loss", a->dtype, a->pairs, a->beta, a->kind, a->label_smoothing);
@@ -265,19 +468,15 @@ extern "C" int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a,
             "pcm_denoise_preference_loss: workspace too small or not 8-byte aligned");
   const PairLoss pl = {a->beta, a->label_smoothing, a->kind};
   const double k = a->mean_reduce ? 1.0 / (double)a->n : 1.0;
-  double* rho = (double*)a->workspace;
   pcm_with_dtype(a->dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    PCM_LAUNCH(denoise_rho_kernel<Dt>, dim3((unsigned)(2 * a->pairs)), dim3(256), 0, stream, (cp)a->pred, (cp)a->ref, (cp)a->target, a->weight, k, rho, a->n);
-    PCM_LAUNCH(pair_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)rho, pl, a->pairs, a->loss, a->log_ratio);
-    if (a->dpred)
-      PCM_LAUNCH(denoise_grad_kernel<Dt>, dim3((unsigned)(2 * a->pairs)), dim3(256), 0, stream, (cp)a->pred, (cp)a->target, a->weight, k, (const double*)rho, pl,
-                 a->grad_scale, (typename Dt::raw*)a->dpred, a->pairs, a->n);
+    const DenoiseRows<Dt> r = {(cp)a->pred, (cp)a->ref, (cp)a->target, a->weight, (typename Dt::raw*)a->dpred, k, a->n};
+    pair_launch(r, (double*)a->workspace, pl, a->grad_scale, a->loss, a->log_ratio, a->pairs, a->n, stream);
   });
   return pcm_post_launch("pcm_denoise_preference_loss");
 }
-extern "C" size_t pcm_preference_loss_workspace_bytes(long pairs, long cols) { return pairs > 0 && cols > 0 ? 4 * (size_t)pairs * sizeof(double) : 0; }
+extern "C" size_t pcm_preference_loss_workspace_bytes(long pairs, long cols) { return pairs > 0 && cols > 0 ? pair_ws_bytes(2 * pairs, cols, 4, TokenRows<DtF32>::SUMS) : 0; }
 extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   PCM_CHECK(a && a->logp && a->ref_logp && a->loss && a->log_ratio && a->cols > 0, PCM_EINVAL, "pcm_preference_loss: null/empty");
   const int rc = pair_args_ok("pcm_preference_loss", a->dtype, a->pairs, a->beta, a->kind, a->label_smoothing);
@@ -288,17 +487,11 @@ extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
             "pcm_preference_loss: workspace too small or not 8-byte aligned");
   const PairLoss pl = {a->beta, a->label_smoothing, a->kind};
   const Places pc = {a->mask, a->ld_mask, a->lengths, a->lengths_i64, a->cols};
-  double* rho = (double*)a->workspace;
-  double* share = rho + 2 * a->pairs;
   pcm_with_dtype(a->dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    PCM_LAUNCH(preference_rho_kernel<Dt>, dim3((unsigned)(2 * a->pairs)), dim3(256), 0, stream, (cp)a->logp, a->ld_logp, (cp)a->ref_logp, a->ld_ref, pc,
-               a->mean_reduce, rho, share);
-    PCM_LAUNCH(pair_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)rho, pl, a->pairs, a->loss, a->log_ratio);
-    if (a->dlogp)
-      PCM_LAUNCH(preference_grad_kernel<Dt>, dim3((unsigned)(2 * a->pairs)), dim3(256), 0, stream, pc, (const double*)rho, (const double*)share, pl,
-                 a->grad_scale, (typename Dt::raw*)a->dlogp, a->ld_dlogp, a->pairs);
+    const TokenRows<Dt> r = {(cp)a->logp, a->ld_logp, (cp)a->ref_logp, a->ld_ref, pc, (typename Dt::raw*)a->dlogp, a->ld_dlogp, a->mean_reduce};
+    pair_launch(r, (double*)a->workspace, pl, a->grad_scale, a->loss, a->log_ratio, a->pairs, a->cols, stream);
   });
   return pcm_post_launch("pcm_preference_loss");
 }

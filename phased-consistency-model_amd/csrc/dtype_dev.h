@@ -3,15 +3,19 @@
 #pragma once
 #include "pcm_common.h"
 
+// VEC: elements of a 16-byte access.  `vec` has the alignment of one element only: rows of odd length and slices of flat buffers start anywhere, and
+// gfx950 takes a 16-byte global access at any element address (hipcc emits global_load_dwordx4 for this type).
 struct DtF32 {
   typedef float raw;
-  static constexpr int VEC = 4;      // elements of a 16-byte access
+  static constexpr int VEC = 4;
+  typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
   static __device__ __forceinline__ float ld(raw r) { return r; }
   static __device__ __forceinline__ raw st(float f) { return f; }
 };
 struct DtBf16 {
   typedef unsigned short raw;
   static constexpr int VEC = 8;
+  typedef unsigned short vec __attribute__((ext_vector_type(8), aligned(2)));
   static __device__ __forceinline__ float ld(raw r) { return __uint_as_float(((unsigned)r) << 16); }
   static __device__ __forceinline__ raw st(float f) {        // round to nearest even, NaN kept quiet
 #ifdef PCM_HOST_EMU
@@ -26,6 +30,7 @@ struct DtBf16 {
 struct DtF16 {
   typedef unsigned short raw;
   static constexpr int VEC = 8;
+  typedef unsigned short vec __attribute__((ext_vector_type(8), aligned(2)));
 #ifdef PCM_HOST_EMU
   static __device__ __forceinline__ float ld(raw r) { return pcm_emu::half_to_float(r); }
   static __device__ __forceinline__ raw st(float f) { return pcm_emu::float_to_half(f); }
@@ -44,11 +49,44 @@ static inline void pcm_with_dtype(int dt, F&& f) {
 static inline bool pcm_dt_ok(int dt) { return dt == PCM_DT_F32 || dt == PCM_DT_BF16 || dt == PCM_DT_F16; }
 static inline size_t pcm_dt_size(int dt) { return dt == PCM_DT_F32 ? 4 : 2; }
 
+// a group of VEC elements at p: all of them (a 16-byte access) or the first `left`, the others 0
+template <typename Dt>
+__device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, float (&v)[Dt::VEC]) {
+  const typename Dt::vec r = *(const typename Dt::vec*)p;
+#pragma unroll
+  for (int j = 0; j < Dt::VEC; j++) v[j] = Dt::ld(r[j]);
+}
+template <typename Dt>
+__device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, long left, float (&v)[Dt::VEC]) {
+  if (left >= Dt::VEC) { pcm_ld_group<Dt>(p, v); return; }
+#pragma unroll
+  for (int j = 0; j < Dt::VEC; j++) v[j] = j < left ? Dt::ld(p[j]) : 0.f;
+}
+template <typename Dt>
+__device__ __forceinline__ void pcm_st_group(typename Dt::raw* p, long left, const float (&v)[Dt::VEC]) {
+  if (left >= Dt::VEC) {
+    typename Dt::vec r;
+#pragma unroll
+    for (int j = 0; j < Dt::VEC; j++) r[j] = Dt::st(v[j]);
+    *(typename Dt::vec*)p = r;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < Dt::VEC; j++)
+    if (j < left) p[j] = Dt::st(v[j]);
+}
+
 // sum over a workgroup of NT threads in a fixed order (wave tree, then the wave sums in wave order), returned to every thread.  `red` holds one
 // value per wave; the barriers at both ends let one buffer serve several sums.
+template <typename V>
+__device__ __forceinline__ V pcm_lane_sum(V v) {      // over the lanes of a wave
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
 template <int NT, typename V>
 __device__ __forceinline__ V pcm_block_sum(V v, V* red) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  v = pcm_lane_sum(v);
   if constexpr (NT == 64) return v;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
