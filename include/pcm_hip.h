@@ -547,25 +547,20 @@ size_t pcm_policy_loss_workspace_bytes(long rows, long cols);
 int pcm_policy_loss(const pcm_policy_args* a, void* stream);
 /* Global norm of gradients held in many tensors, and their clipping (torch.nn.utils' rule, as in pcm_adamw_clip_step):
  *   sumsq = sum g^2 (fp64), norm = sqrt(sumsq);   dst = src * min(1, max_norm / (norm + 1e-6))
- * descs / chunks are tables in DEVICE memory: tensor t is descs[t] and is cut into chunks {t, start} with start = 0, PCM_GRAD_CHUNK, ... < n.
- * dst may be src (then nothing is written when nothing has to be clipped) or a tensor apart; its format may be another one.
- * sumsq is what pcm_adamw_clip_step takes as gradsq. */
+ * `chunks` is a table in DEVICE memory: the tensors cut into pieces of n <= PCM_GRAD_CHUNK consecutive elements, `total` elements in all.
+ * dst may be src (then nothing is written when nothing has to be clipped) or a place apart; its format may be another one.  Pieces that are
+ * written must not overlap one another or any other piece that is read.  sumsq is what pcm_adamw_clip_step takes as gradsq. */
 #define PCM_GRAD_CHUNK 16384
 typedef struct {
   const void* src;
   void* dst;
-  long n;
-  int src_dtype, dst_dtype;
-} pcm_grad_desc;
-typedef struct {
-  long start;
-  long tensor;
+  int n, src_dtype, dst_dtype, unused;
 } pcm_grad_chunk;
-size_t pcm_grad_norm_workspace_bytes(int nchunks);
-int pcm_grad_norm(const pcm_grad_desc* descs, const pcm_grad_chunk* chunks, int nchunks, float* norm, double* sumsq, void* workspace,
+size_t pcm_grad_norm_workspace_bytes(int nchunks, long total);
+int pcm_grad_norm(const pcm_grad_chunk* chunks, int nchunks, long total, float* norm, double* sumsq, void* workspace, size_t workspace_bytes,
+                  void* stream);
+int pcm_grad_clip(const pcm_grad_chunk* chunks, int nchunks, long total, double max_norm, float* norm, double* sumsq, void* workspace,
                   size_t workspace_bytes, void* stream);
-int pcm_grad_clip(const pcm_grad_desc* descs, const pcm_grad_chunk* chunks, int nchunks, double max_norm, float* norm, double* sumsq,
-                  void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -6,23 +6,8 @@
 // caller's workspace, added up by index), so results are bitwise the same run to run.
 #include "dtype_dev.h"
 
-#define AL_LOOP(i, n) for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < (n); i += (long)gridDim.x * blockDim.x)
 static inline int al_blocks(long n) { long b = (n + 255) / 256; return (int)(b > PCM_GRID_CAP(2048) ? PCM_GRID_CAP(2048) : (b < 1 ? 1 : b)); }
 
-// ---- work of one team (a wave or a workgroup of NT threads) on elements [i0, i1) of a row, U groups of 16 bytes per thread in flight ----
-// f(idx, left): the group of VEC elements at idx, `left` of them inside the range (>= VEC: all)
-template <typename Dt, int NT, int U, typename Load, typename Use>
-__device__ __forceinline__ void al_groups(long i0, long i1, int tid, Load&& load, Use&& use) {
-  constexpr long STEP = (long)NT * Dt::VEC;
-  long i = i0 + (long)tid * Dt::VEC;
-  for (; i + (U - 1) * STEP + Dt::VEC <= i1; i += U * STEP) {
-#pragma unroll
-    for (int u = 0; u < U; u++) load(u, i + u * STEP, (long)Dt::VEC);
-#pragma unroll
-    for (int u = 0; u < U; u++) use(u, i + u * STEP, (long)Dt::VEC);
-  }
-  for (; i < i1; i += STEP) { load(0, i, i1 - i); use(0, i, i1 - i); }
-}
 // how a launch cuts rows of n elements: teams of 64 (four rows to a workgroup) for short rows, else `chunks` workgroups of 256 per row, so that some
 // 2048 workgroups (8 per CU) share the work; at most 64 chunks, whose partial sums one wave adds up with one load per lane.
 struct RowCut { int team, chunks; long len; };
@@ -61,7 +46,7 @@ __global__ __launch_bounds__(256) void transition_fwd_kernel(const typename Dt::
   const typename Dt::raw *xr = x + row * n, *mr = mean + row * n;
   float a[4][Dt::VEC], b[4][Dt::VEC];
   double acc = 0.0;
-  al_groups<Dt, TEAM, 4>(i0, i1, tid,
+  pcm_groups<Dt, TEAM, 4>(i0, i1, tid,
     [&](int u, long i, long left) { pcm_ld_group<Dt>(xr + i, left, a[u]); pcm_ld_group<Dt>(mr + i, left, b[u]); },
     [&](int u, long i, long left) {
       float t = 0.f;
@@ -93,7 +78,7 @@ __global__ __launch_bounds__(256) void transition_bwd_kernel(const typename Dt::
   const double s = (double)std[row];
   const float f = (float)((double)dlogp[row] / (s * s * (mean_reduce ? (double)n : 1.0)));
   float a[4][Dt::VEC], b[4][Dt::VEC];
-  al_groups<Dt, TEAM, 4>(i0, i1, tid,
+  pcm_groups<Dt, TEAM, 4>(i0, i1, tid,
     [&](int u, long i, long left) { pcm_ld_group<Dt>(xr + i, left, a[u]); pcm_ld_group<Dt>(mr + i, left, b[u]); },
     [&](int u, long i, long left) {
 #pragma unroll
@@ -139,7 +124,7 @@ struct DenoiseRows {
     const long o = row * n;
     float t[4][Dt::VEC], p[4][Dt::VEC], r[4][Dt::VEC];
     double s = 0.0;
-    al_groups<Dt, NT, 4>(i0, i1, tid,
+    pcm_groups<Dt, NT, 4>(i0, i1, tid,
       [&](int u, long i, long left) {
         pcm_ld_group<Dt>(target + o + i, left, t[u]); pcm_ld_group<Dt>(pred + o + i, left, p[u]); pcm_ld_group<Dt>(ref + o + i, left, r[u]);
       },
@@ -155,7 +140,7 @@ struct DenoiseRows {
   __device__ __forceinline__ void grad(long row, long i0, long i1, int tid, float f) const {
     const long o = row * n;
     float t[4][Dt::VEC], p[4][Dt::VEC];
-    al_groups<Dt, NT, 4>(i0, i1, tid,
+    pcm_groups<Dt, NT, 4>(i0, i1, tid,
       [&](int u, long i, long left) { pcm_ld_group<Dt>(target + o + i, left, t[u]); pcm_ld_group<Dt>(pred + o + i, left, p[u]); },
       [&](int u, long i, long left) {
 #pragma unroll
@@ -221,7 +206,7 @@ struct TokenRows {
     unsigned in[2];
     double s = 0.0;
     int cnt = 0;
-    al_groups<Dt, NT, 2>(i0, len < i1 ? len : i1, tid,
+    pcm_groups<Dt, NT, 2>(i0, len < i1 ? len : i1, tid,
       [&](int u, long i, long left) {
         in[u] = pc.bits<Dt::VEC>(row, i, len);
         pcm_ld_group<Dt>(lr + i, left, a[u]); pcm_ld_group<Dt>(rr + i, left, b[u]);
@@ -238,7 +223,7 @@ struct TokenRows {
   __device__ __forceinline__ void grad(long row, long i0, long i1, int tid, float f) const {
     const long len = pc.len(row);
     unsigned in[2];
-    al_groups<Dt, NT, 2>(i0, i1, tid,
+    pcm_groups<Dt, NT, 2>(i0, i1, tid,
       [&](int u, long i, long left) { in[u] = pc.bits<Dt::VEC>(row, i, len); },
       [&](int u, long i, long left) {
         float g[Dt::VEC];
@@ -356,58 +341,168 @@ __device__ __forceinline__ void policy_place(const PolicyConst c, float lp, floa
     *slope -= c.kl * (k + d);        // exp(d) - 1 = k + d
   }
 }
-// counts per row
-__global__ __launch_bounds__(256) void policy_count_kernel(Places pc, double* count) {
-  __shared__ long red[4];
-  const long row = blockIdx.x, len = pc.len(row);
-  long cnt = 0;
-  for (long c = threadIdx.x; c < len; c += 256) cnt += (!pc.mask || pc.mask[row * pc.ld_mask + c]) ? 1 : 0;
-  cnt = pcm_block_sum<256>(cnt, red);
-  if (threadIdx.x == 0) count[row] = (double)cnt;
+template <typename Dt_>
+struct PolicyRows {
+  typedef Dt_ Dt;
+  typedef typename Dt::raw raw;
+  const raw *logp, *old, *ref;      // old / ref may be NULL
+  long ld_logp, ld_old, ld_ref;
+  const float* adv;
+  long ld_adv;                      // 0: one per row
+  Places pc;
+  PolicyConst con;
+  raw* dlogp;                       // NULL: no gradient
+  long ld_d, rows;
+  float gscale;
+  int reduce;
+};
+struct PolicySums { double obj, kl, held, count; };
+// Groups of VEC places inside a row, numbered row by row; the thread takes g, g + step, ... and keeps (row, group of the row) by addition.  Groups in which
+// nothing counts read nothing.  weight(row, len) is the row's weight in the loss.
+template <typename Dt, typename W>
+__device__ __forceinline__ void policy_groups(const PolicyRows<Dt>& a, long g, long step, W&& weight, PolicySums& s) {
+  constexpr int V = Dt::VEC;
+  const long cols = a.pc.cols, gpr = (cols + V - 1) / V, drow = step / gpr, dcol = step - drow * gpr;
+  long row = g / gpr, col = g - row * gpr;
+  while (row < a.rows) {
+    const long c = col * V, left = cols - c, len = a.pc.len(row);
+    const unsigned in = a.pc.template bits<V>(row, c, len);
+    float out[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) out[j] = 0.f;
+    if (in) {
+      float lp[V], old[V], ref[V], adv[V];
+      pcm_ld_group<Dt>(a.logp + row * a.ld_logp + c, left, lp);
+      if (a.old) pcm_ld_group<Dt>(a.old + row * a.ld_old + c, left, old);
+      if (a.ref) pcm_ld_group<Dt>(a.ref + row * a.ld_ref + c, left, ref);
+      if (a.ld_adv) pcm_ld_group<DtF32>(a.adv + row * a.ld_adv + c, left, adv);
+      else {
+        const float one = a.adv[row];
+#pragma unroll
+        for (int j = 0; j < V; j++) adv[j] = one;
+      }
+      const double w = weight(row, len);
+      const float wg = (float)(w * (double)a.gscale);
+      float so = 0.f, sk = 0.f;
+      int held = 0;
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float obj, kl, slope;
+        bool clipped;
+        policy_place(a.con, lp[j], a.old ? old[j] : lp[j], a.ref != nullptr, a.ref ? ref[j] : 0.f, adv[j], &obj, &kl, &slope, &clipped);
+        const bool counts = in >> j & 1u;
+        so += counts ? obj : 0.f;
+        sk += counts ? kl : 0.f;
+        held += counts && clipped ? 1 : 0;
+        out[j] = counts ? slope * wg : 0.f;
+      }
+      s.obj += w * (double)so; s.kl += w * (double)sk; s.held += (double)held; s.count += (double)__builtin_popcount(in);
+    }
+    if (a.dlogp) pcm_st_group<Dt>(a.dlogp + row * a.ld_d + c, left, out);
+    col += dcol; row += drow;
+    if (col >= gpr) { col -= gpr; row++; }
+  }
 }
-// total[0] = sum of the counts
-__global__ __launch_bounds__(256) void policy_total_kernel(const double* count, long rows, double* total) {
-  __shared__ double red[4];
-  double acc = 0.0;
-  for (long r = threadIdx.x; r < rows; r += 256) acc += count[r];
-  acc = pcm_block_sum<256>(acc, red);
-  if (threadIdx.x == 0) total[0] = acc;
+// how many places count, where the launch has to find out: per row (mean of row means) or in all, as partial sums over groups of 16 places
+__device__ __forceinline__ long count_groups(const Places& pc, long rows, long g, long step) {
+  const long gpr = (pc.cols + 15) / 16, drow = step / gpr, dcol = step - drow * gpr;
+  long row = g / gpr, col = g - row * gpr, n = 0;
+  while (row < rows) {
+    n += __builtin_popcount(pc.bits<16>(row, col * 16, pc.len(row)));
+    col += dcol; row += drow;
+    if (col >= gpr) { col -= gpr; row++; }
+  }
+  return n;
+}
+__global__ __launch_bounds__(256) void policy_count_kernel(Places pc, long rows, double* part) {
+  __shared__ long red[4];
+  long n = 0;
+  if (pc.mask) n = count_groups(pc, rows, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256);
+  else for (long r = (long)blockIdx.x * 256 + threadIdx.x; r < rows; r += (long)gridDim.x * 256) n += pc.len(r);
+  n = pcm_block_sum<256>(n, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = (double)n;
+}
+template <int TEAM>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void policy_count_rows_kernel(Places pc, long rows, double* count) {
+  __shared__ long red[16];
+  const long row = TEAM == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= rows) return;
+  const int tid = TEAM == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const long len = pc.len(row);
+  long n = 0;
+  for (long c = tid * 16L; c < len; c += TEAM * 16L) n += __builtin_popcount(pc.bits<16>(row, c, len));
+  n = pcm_block_sum<TEAM>(n, red);
+  if (tid == 0) count[row] = (double)n;
+}
+// where the number of places comes from: the launch's arguments, partial sums of a launch before, or the lengths themselves
+struct PolicyCount { double known; const double* part; int nparts; const double* per_row; };
+template <typename Dt, int NT>
+__device__ __forceinline__ void policy_part(const PolicyRows<Dt>& a, const PolicyCount& pn, long g, long step, double* red, PolicySums& s) {
+  s.obj = s.kl = s.held = s.count = 0.0;
+  if (a.reduce == PCM_POLICY_TOKEN) {
+    double n = pn.known;
+    if (pn.part) {
+      n = 0.0;
+      for (int i = threadIdx.x; i < pn.nparts; i += NT) n += pn.part[i];
+      n = pcm_block_sum<NT>(n, red);
+    } else if (n < 0.0) {
+      long t = 0;
+      for (long r = threadIdx.x; r < a.rows; r += NT) t += a.pc.len(r);
+      n = pcm_block_sum<NT>((double)t, red);
+    }
+    const double w = 1.0 / fmax(n, 1.0);
+    policy_groups(a, g, step, [&](long, long) { return w; }, s);
+  } else if (a.reduce == PCM_POLICY_ROW) {
+    policy_groups(a, g, step, [&](long row, long len) { return 1.0 / ((pn.per_row ? pn.per_row[row] : (double)len) * (double)a.rows); }, s);
+  } else {
+    policy_groups(a, g, step, [&](long, long) { return 1.0; }, s);
+  }
+  s.obj = pcm_block_sum<NT>(s.obj, red); s.kl = pcm_block_sum<NT>(s.kl, red);
+  s.held = pcm_block_sum<NT>(s.held, red); s.count = pcm_block_sum<NT>(s.count, red);
+}
+__device__ __forceinline__ void policy_result(const PolicySums& s, double kl, float* loss, float* stats) {
+  loss[0] = (float)(s.obj + kl * s.kl);
+  stats[0] = (float)s.obj; stats[1] = (float)s.kl; stats[2] = (float)(s.held / fmax(s.count, 1.0)); stats[3] = (float)s.count;
 }
 template <typename Dt>
-__global__ __launch_bounds__(256) void policy_main_kernel(const typename Dt::raw* logp, long ld_logp, const typename Dt::raw* old, long ld_old,
-                                                          const typename Dt::raw* ref, long ld_ref, const float* adv, long ld_adv, int adv_row, Places pc,
-                                                          PolicyConst con, int reduce, float gscale, const double* count, const double* total,
-                                                          typename Dt::raw* dlogp, long ld_d, long rows, double* part) {
+__global__ __launch_bounds__(256) void policy_main_kernel(PolicyRows<Dt> a, PolicyCount pn, double* part) {
   __shared__ double red[4];
-  const double inv_total = 1.0 / fmax(total[0], 1.0);
-  double so = 0.0, sk = 0.0, sc = 0.0;
-  AL_LOOP(i, rows * pc.cols) {
-    const long row = i / pc.cols, c = i - row * pc.cols;
-    float g = 0.f;
-    if (c < pc.len(row) && (!pc.mask || pc.mask[row * pc.ld_mask + c])) {
-      const double w = reduce == PCM_POLICY_TOKEN ? inv_total : (reduce == PCM_POLICY_ROW ? 1.0 / (count[row] * (double)rows) : 1.0);
-      const float lp = Dt::ld(logp[row * ld_logp + c]);
-      float obj, kl, slope;
-      bool clipped;
-      policy_place(con, lp, old ? Dt::ld(old[row * ld_old + c]) : lp, ref != nullptr, ref ? Dt::ld(ref[row * ld_ref + c]) : 0.f,
-                   adv[adv_row ? row : row * ld_adv + c], &obj, &kl, &slope, &clipped);
-      so += w * (double)obj; sk += w * (double)kl; sc += clipped ? 1.0 : 0.0;
-      g = slope * (float)(w * (double)gscale);
-    }
-    if (dlogp) dlogp[row * ld_d + c] = Dt::st(g);
-  }
-  so = pcm_block_sum<256>(so, red); sk = pcm_block_sum<256>(sk, red); sc = pcm_block_sum<256>(sc, red);
-  if (threadIdx.x == 0) { part[3 * blockIdx.x] = so; part[3 * blockIdx.x + 1] = sk; part[3 * blockIdx.x + 2] = sc; }
+  PolicySums s;
+  policy_part<Dt, 256>(a, pn, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, red, s);
+  if (threadIdx.x == 0) { double* q = part + 4 * (long)blockIdx.x; q[0] = s.obj; q[1] = s.kl; q[2] = s.held; q[3] = s.count; }
 }
-__global__ __launch_bounds__(256) void policy_finish_kernel(const double* part, int nparts, const double* total, double kl, float* loss, float* stats) {
+__global__ __launch_bounds__(256) void policy_finish_kernel(const double* part, int nparts, double kl, float* loss, float* stats) {
   __shared__ double red[4];
-  double so = 0.0, sk = 0.0, sc = 0.0;
-  for (int i = threadIdx.x; i < nparts; i += 256) { so += part[3 * i]; sk += part[3 * i + 1]; sc += part[3 * i + 2]; }
-  so = pcm_block_sum<256>(so, red); sk = pcm_block_sum<256>(sk, red); sc = pcm_block_sum<256>(sc, red);
-  if (threadIdx.x == 0) {
-    loss[0] = (float)(so + kl * sk);
-    stats[0] = (float)so; stats[1] = (float)sk; stats[2] = (float)(sc / fmax(total[0], 1.0)); stats[3] = (float)total[0];
+  PolicySums s = {0.0, 0.0, 0.0, 0.0};
+  for (int i = threadIdx.x; i < nparts; i += 256) { s.obj += part[4 * i]; s.kl += part[4 * i + 1]; s.held += part[4 * i + 2]; s.count += part[4 * i + 3]; }
+  s.obj = pcm_block_sum<256>(s.obj, red); s.kl = pcm_block_sum<256>(s.kl, red);
+  s.held = pcm_block_sum<256>(s.held, red); s.count = pcm_block_sum<256>(s.count, red);
+  if (threadIdx.x == 0) policy_result(s, kl, loss, stats);
+}
+// few places: one workgroup counts, forms loss and gradient, and adds up, in one launch
+#define POLICY_SMALL_PLACES 16384
+#define POLICY_SMALL_ROWS 2048
+template <typename Dt>
+__global__ __launch_bounds__(1024) void policy_small_kernel(PolicyRows<Dt> a, double kl, float* loss, float* stats) {
+  __shared__ double red[16];
+  __shared__ double per_row[POLICY_SMALL_ROWS];
+  PolicyCount pn = {-1.0, nullptr, 0, nullptr};
+  if (a.pc.mask && a.reduce == PCM_POLICY_TOKEN) {
+    pn.known = pcm_block_sum<1024>((double)count_groups(a.pc, a.rows, threadIdx.x, 1024), red);
+  } else if (a.pc.mask && a.reduce == PCM_POLICY_ROW) {
+    for (long row = threadIdx.x >> 6; row < a.rows; row += 16) {
+      const long len = a.pc.len(row);
+      long n = 0;
+      for (long c = (threadIdx.x & 63) * 16L; c < len; c += 64 * 16L) n += __builtin_popcount(a.pc.template bits<16>(row, c, len));
+      n = pcm_lane_sum(n);
+      if ((threadIdx.x & 63) == 0) per_row[row] = (double)n;
+    }
+    __syncthreads();
+    pn.per_row = per_row;
   }
+  PolicySums s;
+  policy_part<Dt, 1024>(a, pn, threadIdx.x, 1024, red, s);
+  if (threadIdx.x == 0) policy_result(s, kl, loss, stats);
 }
 
 // ---- entry points ----
@@ -495,8 +590,12 @@ extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   });
   return pcm_post_launch("pcm_preference_loss");
 }
+static bool policy_small(long rows, long cols) { return rows <= POLICY_SMALL_ROWS && rows * cols <= POLICY_SMALL_PLACES; }
+static int policy_blocks(long rows, long cols, int vec) { return al_blocks(rows * ((cols + vec - 1) / vec)); }
+#define POLICY_COUNT_PARTS 512
 extern "C" size_t pcm_policy_loss_workspace_bytes(long rows, long cols) {
-  return rows > 0 && cols > 0 ? ((size_t)rows + 1 + 3 * (size_t)al_blocks(rows * cols)) * sizeof(double) : 0;
+  if (rows <= 0 || cols <= 0 || policy_small(rows, cols)) return 0;
+  return ((size_t)(rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS) + 4 * (size_t)policy_blocks(rows, cols, 4)) * sizeof(double);
 }
 extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
   PCM_CHECK(a && a->logp && a->advantages && a->loss && a->stats && a->rows > 0 && a->rows <= AL_MAX_ROWS && a->cols > 0, PCM_EINVAL, "pcm_policy_loss: null/empty");
@@ -506,21 +605,40 @@ extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
   PCM_CHECK(a->kl_coef == 0.0 || a->ref_logp, PCM_EINVAL, "pcm_policy_loss: a KL term needs the reference log-probabilities");
   PCM_CHECK(a->ld_logp >= a->cols && (!a->old_logp || a->ld_old >= a->cols) && (!a->ref_logp || a->ld_ref >= a->cols) && (a->adv_per_row || a->ld_adv >= a->cols) &&
                 (!a->mask || a->ld_mask >= a->cols) && (!a->dlogp || a->ld_dlogp >= a->cols), PCM_EINVAL, "pcm_policy_loss: row stride below the row length");
-  PCM_CHECK(a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= pcm_policy_loss_workspace_bytes(a->rows, a->cols), PCM_EINVAL,
+  const size_t need = pcm_policy_loss_workspace_bytes(a->rows, a->cols);
+  PCM_CHECK(need == 0 || (a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= need), PCM_EINVAL,
             "pcm_policy_loss: workspace too small or not 8-byte aligned");
   const Places pc = {a->mask, a->ld_mask, a->lengths, a->lengths_i64, a->cols};
   const PolicyConst con = {log1p(a->clip_high), log1p(-a->clip_low), (float)(1.0 + a->clip_high), (float)(1.0 - a->clip_low), (float)a->kl_coef};
-  double *count = (double*)a->workspace, *total = count + a->rows, *part = total + 1;
-  const int nb = al_blocks(a->rows * a->cols);
-  PCM_LAUNCH(policy_count_kernel, dim3((unsigned)a->rows), dim3(256), 0, stream, pc, count);
-  PCM_LAUNCH(policy_total_kernel, dim3(1), dim3(256), 0, stream, (const double*)count, a->rows, total);
+  const long rows = a->rows;
+  const int reduce = a->reduce == PCM_POLICY_ROW && rows == 1 ? PCM_POLICY_TOKEN : a->reduce;      // one row: its mean is the mean of all places
   pcm_with_dtype(a->dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    PCM_LAUNCH(policy_main_kernel<Dt>, dim3(nb), dim3(256), 0, stream, (cp)a->logp, a->ld_logp, (cp)a->old_logp, a->ld_old, (cp)a->ref_logp, a->ld_ref,
-               a->advantages, a->ld_adv, a->adv_per_row, pc, con, a->reduce, (float)a->grad_scale, (const double*)count, (const double*)total,
-               (typename Dt::raw*)a->dlogp, a->ld_dlogp, a->rows, part);
+    const PolicyRows<Dt> r = {(cp)a->logp, (cp)a->old_logp, (cp)a->ref_logp, a->ld_logp, a->ld_old, a->ld_ref, a->advantages, a->adv_per_row ? 0 : a->ld_adv, pc, con,
+                              (typename Dt::raw*)a->dlogp, a->ld_dlogp, rows, (float)a->grad_scale, reduce};
+    if (need == 0) {
+      PCM_LAUNCH(policy_small_kernel<Dt>, dim3(1), dim3(1024), 0, stream, r, a->kl_coef, a->loss, a->stats);
+      return;
+    }
+    double *counts = (double*)a->workspace, *part = counts + (rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS);
+    PolicyCount pn = {-1.0, nullptr, 0, nullptr};
+    if (reduce == PCM_POLICY_TOKEN) {
+      if (!a->mask && !a->lengths) pn.known = (double)rows * (double)a->cols;
+      else if (a->mask || rows > 4096) {          // (up to 4096 lengths each workgroup adds up itself: 16 loads a thread against a launch)
+        const long b = a->mask ? al_blocks(rows * ((a->cols + 15) / 16)) : al_blocks(rows);
+        pn.nparts = (int)(b < POLICY_COUNT_PARTS ? b : POLICY_COUNT_PARTS);
+        pn.part = counts;
+        PCM_LAUNCH(policy_count_kernel, dim3(pn.nparts), dim3(256), 0, stream, pc, rows, counts);
+      }
+    } else if (reduce == PCM_POLICY_ROW && a->mask) {
+      pn.per_row = counts;
+      if (a->cols <= 4096) PCM_LAUNCH(policy_count_rows_kernel<64>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, pc, rows, counts);
+      else PCM_LAUNCH(policy_count_rows_kernel<1024>, dim3((unsigned)rows), dim3(1024), 0, stream, pc, rows, counts);
+    }
+    const int nb = policy_blocks(rows, a->cols, Dt::VEC);
+    PCM_LAUNCH(policy_main_kernel<Dt>, dim3(nb), dim3(256), 0, stream, r, pn, part);
+    PCM_LAUNCH(policy_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)part, nb, a->kl_coef, a->loss, a->stats);
   });
-  PCM_LAUNCH(policy_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)part, nb, (const double*)total, a->kl_coef, a->loss, a->stats);
   return pcm_post_launch("pcm_policy_loss");
 }

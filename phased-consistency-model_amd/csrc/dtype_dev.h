@@ -3,19 +3,17 @@
 #pragma once
 #include "pcm_common.h"
 
-// VEC: elements of a 16-byte access.  `vec` has the alignment of one element only: rows of odd length and slices of flat buffers start anywhere, and
-// gfx950 takes a 16-byte global access at any element address (hipcc emits global_load_dwordx4 for this type).
+// VEC: elements of a 16-byte access.  The vector types below have the alignment of one element only: rows of odd length and slices of flat buffers
+// start anywhere, and gfx950 takes a 16-byte global access at any element address (hipcc emits global_load_dwordx4 for them).
 struct DtF32 {
   typedef float raw;
   static constexpr int VEC = 4;
-  typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
   static __device__ __forceinline__ float ld(raw r) { return r; }
   static __device__ __forceinline__ raw st(float f) { return f; }
 };
 struct DtBf16 {
   typedef unsigned short raw;
   static constexpr int VEC = 8;
-  typedef unsigned short vec __attribute__((ext_vector_type(8), aligned(2)));
   static __device__ __forceinline__ float ld(raw r) { return __uint_as_float(((unsigned)r) << 16); }
   static __device__ __forceinline__ raw st(float f) {        // round to nearest even, NaN kept quiet
 #ifdef PCM_HOST_EMU
@@ -30,7 +28,6 @@ struct DtBf16 {
 struct DtF16 {
   typedef unsigned short raw;
   static constexpr int VEC = 8;
-  typedef unsigned short vec __attribute__((ext_vector_type(8), aligned(2)));
 #ifdef PCM_HOST_EMU
   static __device__ __forceinline__ float ld(raw r) { return pcm_emu::half_to_float(r); }
   static __device__ __forceinline__ raw st(float f) { return pcm_emu::float_to_half(f); }
@@ -49,31 +46,48 @@ static inline void pcm_with_dtype(int dt, F&& f) {
 static inline bool pcm_dt_ok(int dt) { return dt == PCM_DT_F32 || dt == PCM_DT_BF16 || dt == PCM_DT_F16; }
 static inline size_t pcm_dt_size(int dt) { return dt == PCM_DT_F32 ? 4 : 2; }
 
-// a group of VEC elements at p: all of them (a 16-byte access) or the first `left`, the others 0
-template <typename Dt>
-__device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, float (&v)[Dt::VEC]) {
-  const typename Dt::vec r = *(const typename Dt::vec*)p;
+// a group of N elements at p (N deduced from v): all of them in one access, or the first `left` and 0 for the others
+template <typename Dt, int N>
+__device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, float (&v)[N]) {
+  typedef typename Dt::raw vec __attribute__((ext_vector_type(N), aligned(sizeof(typename Dt::raw))));
+  const vec r = *(const vec*)p;
 #pragma unroll
-  for (int j = 0; j < Dt::VEC; j++) v[j] = Dt::ld(r[j]);
+  for (int j = 0; j < N; j++) v[j] = Dt::ld(r[j]);
 }
-template <typename Dt>
-__device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, long left, float (&v)[Dt::VEC]) {
-  if (left >= Dt::VEC) { pcm_ld_group<Dt>(p, v); return; }
+template <typename Dt, int N>
+__device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, long left, float (&v)[N]) {
+  if (left >= N) { pcm_ld_group<Dt>(p, v); return; }
 #pragma unroll
-  for (int j = 0; j < Dt::VEC; j++) v[j] = j < left ? Dt::ld(p[j]) : 0.f;
+  for (int j = 0; j < N; j++) v[j] = j < left ? Dt::ld(p[j]) : 0.f;
 }
-template <typename Dt>
-__device__ __forceinline__ void pcm_st_group(typename Dt::raw* p, long left, const float (&v)[Dt::VEC]) {
-  if (left >= Dt::VEC) {
-    typename Dt::vec r;
+template <typename Dt, int N>
+__device__ __forceinline__ void pcm_st_group(typename Dt::raw* p, long left, const float (&v)[N]) {
+  if (left >= N) {
+    typedef typename Dt::raw vec __attribute__((ext_vector_type(N), aligned(sizeof(typename Dt::raw))));
+    vec r;
 #pragma unroll
-    for (int j = 0; j < Dt::VEC; j++) r[j] = Dt::st(v[j]);
-    *(typename Dt::vec*)p = r;
+    for (int j = 0; j < N; j++) r[j] = Dt::st(v[j]);
+    *(vec*)p = r;
     return;
   }
 #pragma unroll
-  for (int j = 0; j < Dt::VEC; j++)
+  for (int j = 0; j < N; j++)
     if (j < left) p[j] = Dt::st(v[j]);
+}
+
+// ---- work of one team (a wave or a workgroup of NT threads) on elements [i0, i1) of a row, U groups of 16 bytes per thread in flight ----
+// f(idx, left): the group of VEC elements at idx, `left` of them inside the range (>= VEC: all)
+template <typename Dt, int NT, int U, typename Load, typename Use>
+__device__ __forceinline__ void pcm_groups(long i0, long i1, int tid, Load&& load, Use&& use) {
+  constexpr long STEP = (long)NT * Dt::VEC;
+  long i = i0 + (long)tid * Dt::VEC;
+  for (; i + (U - 1) * STEP + Dt::VEC <= i1; i += U * STEP) {
+#pragma unroll
+    for (int u = 0; u < U; u++) load(u, i + u * STEP, (long)Dt::VEC);
+#pragma unroll
+    for (int u = 0; u < U; u++) use(u, i + u * STEP, (long)Dt::VEC);
+  }
+  for (; i < i1; i += STEP) { load(0, i, i1 - i); use(0, i, i1 - i); }
 }
 
 // sum over a workgroup of NT threads in a fixed order (wave tree, then the wave sums in wave order), returned to every thread.  `red` holds one

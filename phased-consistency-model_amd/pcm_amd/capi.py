@@ -169,8 +169,8 @@ _PROTOS = {
     "pcm_denoise_preference_loss": [C.POINTER(DenoisePreferenceArgs), vp],
     "pcm_preference_loss": [C.POINTER(PreferenceArgs), vp],
     "pcm_policy_loss": [C.POINTER(PolicyArgs), vp],
-    "pcm_grad_norm": [vp, vp, i32, vp, vp, vp, C.c_size_t, vp],
-    "pcm_grad_clip": [vp, vp, i32, C.c_double, vp, vp, vp, C.c_size_t, vp],
+    "pcm_grad_norm": [vp, i32, i64, vp, vp, vp, C.c_size_t, vp],
+    "pcm_grad_clip": [vp, i32, i64, C.c_double, vp, vp, vp, C.c_size_t, vp],
 }
 
 
@@ -230,7 +230,7 @@ class Lib:
                            ("pcm_mod_grad_workspace_bytes", [C.c_int] * 3),        # abi 5
                            ("pcm_transition_logprob_workspace_bytes", [C.c_long] * 2), ("pcm_denoise_preference_loss_workspace_bytes", [C.c_long] * 2),
                            ("pcm_preference_loss_workspace_bytes", [C.c_long] * 2), ("pcm_policy_loss_workspace_bytes", [C.c_long] * 2),
-                           ("pcm_grad_norm_workspace_bytes", [C.c_int])):        # abi 6
+                           ("pcm_grad_norm_workspace_bytes", [C.c_int, C.c_long])):        # abi 6
             f = getattr(self.dll, name, None)
             if f is not None:
                 f.restype, f.argtypes = C.c_size_t, argt

@@ -1054,17 +1054,18 @@ class GradSet:
             end_any = max(end_any, b)
             end_out = max(end_out, b) if is_out else end_out
         self._keep = (grads, dsts)
-        desc = np.array(rows, dtype=[("src", "<u8"), ("dst", "<u8"), ("n", "<i8"), ("sdt", "<i4"), ("ddt", "<i4")])
-        per = (desc["n"] + capi.GRAD_CHUNK - 1) // capi.GRAD_CHUNK
-        self.chunks = int(per.sum())
+        src, dst, n, sdt, ddt = np.array(rows, dtype=np.int64).reshape(-1, 5).T
+        per = (n + capi.GRAD_CHUNK - 1) // capi.GRAD_CHUNK
+        self.chunks, self.total = int(per.sum()), int(n.sum())
         if self.chunks >= 2 ** 31:
             raise ValueError("GradSet: too many elements")
-        tensor = np.repeat(np.arange(len(rows)), per)
-        first = np.repeat(np.cumsum(per) - per, per)
-        chunk = np.stack([(np.arange(self.chunks) - first) * capi.GRAD_CHUNK, tensor], axis=1).astype("<i8")
-        self._cut = desc.nbytes
-        table = np.concatenate([np.frombuffer(desc.tobytes(), np.uint8), np.frombuffer(chunk.tobytes(), np.uint8)])
-        self._table = torch.from_numpy(table.copy()).to(self.device)
+        t = np.repeat(np.arange(len(rows)), per)                                             # tensor of each piece, and its first element
+        start = (np.arange(self.chunks) - np.repeat(np.cumsum(per) - per, per)) * capi.GRAD_CHUNK
+        size = np.array([4, 2, 2])                                                           # bytes of an element by PCM_DT_* code
+        table = np.zeros(self.chunks, dtype=[("src", "<i8"), ("dst", "<i8"), ("n", "<i4"), ("sdt", "<i4"), ("ddt", "<i4"), ("unused", "<i4")])
+        table["src"], table["dst"] = src[t] + start * size[sdt[t]], dst[t] + start * size[ddt[t]]
+        table["n"], table["sdt"], table["ddt"] = np.minimum(n[t] - start, capi.GRAD_CHUNK), sdt[t], ddt[t]
+        self._table = torch.from_numpy(table.view(np.uint8)).to(self.device)
         self._stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
 
     def _run(self, name, sumsq, *more):
@@ -1077,10 +1078,9 @@ class GradSet:
             sumsq.zero_()
             return torch.zeros(1, dtype=torch.float32, device=dev)
         norm = torch.empty(1, dtype=torch.float32, device=dev)
-        nb = capi.lib().dll.pcm_grad_norm_workspace_bytes(self.chunks)
+        nb = capi.lib().dll.pcm_grad_norm_workspace_bytes(self.chunks, self.total)
         ws = _scratch(dev, nb)
-        base = self._table.data_ptr()
-        _call_on(dev, name, base, base + self._cut, self.chunks, *more, ptr(norm), ptr(sumsq), ptr(ws), nb)
+        _call_on(dev, name, ptr(self._table), self.chunks, self.total, *more, ptr(norm), ptr(sumsq), ptr(ws), nb)
         if self._stream is not None and not torch.cuda.is_current_stream_capturing():
             now = torch.cuda.current_stream(dev)
             if now != self._stream:
