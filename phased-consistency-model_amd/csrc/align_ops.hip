@@ -9,12 +9,12 @@
 static inline int al_blocks(long n) { long b = (n + 255) / 256; return (int)(b > PCM_GRID_CAP(2048) ? PCM_GRID_CAP(2048) : (b < 1 ? 1 : b)); }
 
 // how a launch cuts rows of n elements: teams of 64 (four rows to a workgroup) for short rows, else `chunks` workgroups of 256 per row, so that some
-// 2048 workgroups (8 per CU) share the work; at most 64 chunks, whose partial sums one wave adds up with one load per lane.
+// 4096 workgroups (two rounds of 8 per CU) share the work; at most 64 chunks, whose partial sums one wave adds up with one load per lane.
 struct RowCut { int team, chunks; long len; };
 static RowCut row_cut(long rows, long n, int vec) {
   RowCut c = {256, 1, n};
   if (n <= 1024) { c.team = 64; return c; }
-  const long unit = 256L * vec, most = (n + unit - 1) / unit, want = 2048 / rows;
+  const long unit = 256L * vec, most = (n + unit - 1) / unit, want = 4096 / rows;
   long k = want < 1 ? 1 : (want < most ? want : most);
   if (k > 64) k = 64;
   c.len = ((n + k - 1) / k + unit - 1) / unit * unit;
@@ -126,7 +126,7 @@ struct DenoiseRows {
     double s = 0.0;
     pcm_groups<Dt, NT, 4>(i0, i1, tid,
       [&](int u, long i, long left) {
-        pcm_ld_group<Dt>(target + o + i, left, t[u]); pcm_ld_group<Dt>(pred + o + i, left, p[u]); pcm_ld_group<Dt>(ref + o + i, left, r[u]);
+        pcm_ld_group<Dt, true>(target + o + i, left, t[u]); pcm_ld_group<Dt, true>(pred + o + i, left, p[u]); pcm_ld_group<Dt, true>(ref + o + i, left, r[u]);
       },
       [&](int u, long i, long left) {
         float e = 0.f;
@@ -141,7 +141,7 @@ struct DenoiseRows {
     const long o = row * n;
     float t[4][Dt::VEC], p[4][Dt::VEC];
     pcm_groups<Dt, NT, 4>(i0, i1, tid,
-      [&](int u, long i, long left) { pcm_ld_group<Dt>(target + o + i, left, t[u]); pcm_ld_group<Dt>(pred + o + i, left, p[u]); },
+      [&](int u, long i, long left) { pcm_ld_group<Dt, true>(target + o + i, left, t[u]); pcm_ld_group<Dt, true>(pred + o + i, left, p[u]); },
       [&](int u, long i, long left) {
 #pragma unroll
         for (int j = 0; j < Dt::VEC; j++) t[u][j] = (t[u][j] - p[u][j]) * f;
@@ -153,6 +153,8 @@ struct DenoiseRows {
   __device__ __forceinline__ double factor(long row, const double (&s)[SUMS]) const { return 2.0 * scale(row); }
   bool wants_grad() const { return dpred != nullptr; }
 };
+// element (row, c) of rows ld apart, both below 2^32 (one 32 x 32 -> 64 bit multiply-add)
+__device__ __forceinline__ long at(long row, long ld, long c) { return (long)((unsigned long)(unsigned)row * (unsigned)ld + (unsigned long)c); }
 // places that count: mask[row][col] != 0 (or no mask) and col < lengths[row] (or no lengths)
 struct Places {
   const unsigned char* mask; long ld_mask;
@@ -163,28 +165,38 @@ struct Places {
     const long v = i64 ? (long)((const int64_t*)lengths)[row] : (long)((const int32_t*)lengths)[row];
     return v < 0 ? 0 : (v > cols ? cols : v);
   }
-  // bit j: place c + j of the row counts, c + j < c + left and < len
+  // bit j of the result: place c + j counts
   template <int VEC>
-  __device__ __forceinline__ unsigned bits(long row, long c, long len) const {
-    const long left = len - c;
-    if (left <= 0) return 0u;
-    unsigned in = left >= VEC ? (1u << VEC) - 1u : (1u << left) - 1u;
+  static __device__ __forceinline__ unsigned below(long left) { return left <= 0 ? 0u : (left >= VEC ? (1u << VEC) - 1u : (1u << left) - 1u); }
+  template <int VEC>
+  __device__ __forceinline__ unsigned bits_inside(long row, long c, long len) const {      // all VEC places are inside the row
+    unsigned got = (1u << VEC) - 1u;
     if (mask) {
-      const unsigned char* m = mask + row * ld_mask + c;
-      unsigned got = 0u;
-      if (left >= VEC) {
-        typedef unsigned char mv __attribute__((ext_vector_type(VEC), aligned(1)));
-        const mv b = *(const mv*)m;
+      typedef unsigned mv __attribute__((ext_vector_type(VEC / 4), aligned(1)));
+      const mv b = *(const mv*)(mask + at(row, ld_mask, c));
+      got = 0u;
 #pragma unroll
-        for (int j = 0; j < VEC; j++) got |= b[j] ? 1u << j : 0u;
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; j++)
-          if (j < left) got |= m[j] ? 1u << j : 0u;
+      for (int w = 0; w < VEC / 4; w++) {
+        // the top bit of a byte that is not 0, then the four of them side by side: 8 j + (24 - 7 j) = 24 + j, the other products fall elsewhere
+        const unsigned x = ((((b[w] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | b[w]) >> 7) & 0x01010101u;
+        got |= (x * 0x01020408u) >> 24 << (4 * w);
       }
-      in &= got;
+    }
+    return got & below<VEC>(len - c);
+  }
+  template <int VEC>
+  __device__ __forceinline__ unsigned bits_end(long row, long c, long len) const {         // the row may end before
+    unsigned in = below<VEC>(len - c);
+    if (mask) {
+#pragma unroll
+      for (int j = 0; j < VEC; j++)
+        if ((in >> j & 1u) && !mask[at(row, ld_mask, c + j)]) in &= ~(1u << j);
     }
     return in;
+  }
+  template <int VEC>
+  __device__ __forceinline__ unsigned bits(long row, long c, long len) const {
+    return c + VEC <= cols ? bits_inside<VEC>(row, c, len) : bits_end<VEC>(row, c, len);
   }
 };
 // log-probabilities: rho = sum (mean) over the places that count of logp - ref;  d rho / d logp = 1 (1 / count) there
@@ -208,7 +220,7 @@ struct TokenRows {
     int cnt = 0;
     pcm_groups<Dt, NT, 2>(i0, len < i1 ? len : i1, tid,
       [&](int u, long i, long left) {
-        in[u] = pc.bits<Dt::VEC>(row, i, len);
+        in[u] = left >= Dt::VEC ? pc.bits_inside<Dt::VEC>(row, i, len) : pc.bits_end<Dt::VEC>(row, i, len);
         pcm_ld_group<Dt>(lr + i, left, a[u]); pcm_ld_group<Dt>(rr + i, left, b[u]);
       },
       [&](int u, long i, long left) {
@@ -224,7 +236,7 @@ struct TokenRows {
     const long len = pc.len(row);
     unsigned in[2];
     pcm_groups<Dt, NT, 2>(i0, i1, tid,
-      [&](int u, long i, long left) { in[u] = pc.bits<Dt::VEC>(row, i, len); },
+      [&](int u, long i, long left) { in[u] = left >= Dt::VEC ? pc.bits_inside<Dt::VEC>(row, i, len) : pc.bits_end<Dt::VEC>(row, i, len); },
       [&](int u, long i, long left) {
         float g[Dt::VEC];
 #pragma unroll
@@ -311,99 +323,170 @@ static void pair_launch(const R& r, double* part, const PairLoss& pl, double gsc
 }
 
 // ---- clipped policy loss with a KL term ----
-// exp(d) - d - 1 to full relative accuracy: below 1/2 the power series d^2/2 (1 + d/3 (1 + d/4 (...))) -- the difference itself would leave
-// nothing of a small d -- with terms to d^10 (the first one left out is 2^-10 * 2 / 12! of the sum); above, the difference.
+// e^x to about two steps: 2^t with t = x log2 e, the product's rounding error e carried along as the factor 1 + e ln 2 (v_exp_f32 alone would be off by
+// |x| half steps).  Half the instructions of expf; results below 2^-126 come out as 0.
+__device__ __forceinline__ float exp_of(float x) {
+  const float hi = 1.44269502162933349609375f, lo = 1.92596299112661746887e-8f;      // log2 e in two fp32 numbers
+  const float t = x * hi, e = fmaf(x, lo, fmaf(x, hi, -t)), r = PCM_EXP2F(t);
+  return fabsf(x) < 100.0f ? r * fmaf(e, 0.693147182464599609375f, 1.0f) : r;        // (beyond, r is 0 or infinite, or x is no number)
+}
+// exp(d) - d - 1 to full relative accuracy: below 1/2 the power series d^2 (1/2! + d/3! + ... + d^7/9!) -- the difference itself would leave nothing
+// of a small d -- whose first term left out is 2 / (10! 2^8) of the sum at the most; above, the difference.
 __device__ __forceinline__ float kl_term(float d) {
   if (fabsf(d) < 0.5f) {
-    float s = 1.0f + d * (1.0f / 10.0f);
-    s = 1.0f + d * (1.0f / 9.0f) * s; s = 1.0f + d * (1.0f / 8.0f) * s; s = 1.0f + d * (1.0f / 7.0f) * s; s = 1.0f + d * (1.0f / 6.0f) * s;
-    s = 1.0f + d * (1.0f / 5.0f) * s; s = 1.0f + d * (1.0f / 4.0f) * s; s = 1.0f + d * (1.0f / 3.0f) * s;
-    return 0.5f * d * d * s;
+    float s = fmaf(d, 1.0f / 362880.0f, 1.0f / 40320.0f);
+    s = fmaf(d, s, 1.0f / 5040.0f); s = fmaf(d, s, 1.0f / 720.0f); s = fmaf(d, s, 1.0f / 120.0f); s = fmaf(d, s, 1.0f / 24.0f);
+    s = fmaf(d, s, 1.0f / 6.0f); s = fmaf(d, s, 0.5f);
+    return d * d * s;
   }
-  return (expf(d) - 1.0f) - d;
+  return (exp_of(d) - 1.0f) - d;
 }
-struct PolicyConst { double log_over, log_under; float over, under, kl; };     // log(1 + hi), log(1 - lo), 1 + hi, 1 - lo, KL coefficient
-// one place: the clipped objective, the KL estimate, the derivative of objective + kl * KL by logp.  The border of the clipping is decided in fp64:
-// the difference of two fp32 numbers is exact there.
-__device__ __forceinline__ void policy_place(const PolicyConst c, float lp, float old, bool has_ref, float ref, float a, float* obj, float* kl,
-                                             float* slope, bool* clipped) {
-  const double x = (double)lp - (double)old;
-  const bool over = a > 0.f && x > c.log_over, under = a < 0.f && x < c.log_under;
-  // (an advantage of zero adds nothing, also where exp leaves fp32; a NaN stays one)
-  const float r = a == 0.f && x == x ? 0.f : expf((float)x);
-  *clipped = over || under;
-  *obj = -a * (over ? c.over : (under ? c.under : r));
-  *slope = *clipped ? 0.f : -a * r;
-  *kl = 0.f;
-  if (has_ref) {
+// log(1 + hi) and log(1 - lo) in fp64 and rounded to fp32, 1 + hi, 1 - lo, KL coefficient
+struct PolicyConst { double log_over, log_under; float log_over_f, log_under_f, over, under, kl; };
+// what a place needs of its advantage a: a bound holds r = e^x where a's sign times x is beyond `border`, and the objective is then `held`
+struct PolicySide {
+  float a, border, held;
+  bool neg, zero;
+  __device__ __forceinline__ PolicySide() {}
+  __device__ __forceinline__ PolicySide(const PolicyConst& c, float adv) {
+    a = adv; neg = adv < 0.f; zero = adv == 0.f;
+    border = zero ? __uint_as_float(0x7f800000u) : (neg ? -c.log_under_f : c.log_over_f);
+    held = -adv * (neg ? c.under : c.over);
+  }
+};
+// one place: the clipped objective, the KL estimate, the derivative of objective + kl * KL by logp.  The side of the border that logp - old_logp is on is that
+// of the exact difference: the rounded one decides unless it falls on the rounded border itself, and then fp64, where the difference of two fp32
+// numbers this close is exact, does.
+template <bool KL>
+__device__ __forceinline__ void policy_place(const PolicyConst& c, const PolicySide& s, float lp, float old, float ref, float* obj, float* kl, float* slope,
+                                             bool* held) {
+  const float x = lp - old, y = s.neg ? -x : x;
+  bool beyond = y > s.border;
+  if (y == s.border) {
+    const double e = (double)lp - (double)old;
+    beyond = !s.zero && (s.neg ? e < c.log_under : e > c.log_over);
+  }
+  // an advantage of zero adds nothing, also where exp leaves fp32 (x - x: 0, or the NaN of a NaN or an infinity)
+  const float ar = s.zero ? x - x : s.a * exp_of(x);
+  *held = beyond;
+  *obj = beyond ? s.held : -ar;
+  *slope = beyond ? 0.f : -ar;
+  if constexpr (KL) {
     const float d = ref - lp, k = kl_term(d);
     *kl = k;
     *slope -= c.kl * (k + d);        // exp(d) - 1 = k + d
   }
 }
+#define POLICY_GROUP 4      /* places of a thread's group in every format (8 need 98 registers: half the waves, 59 us against 50 at 2048 x 8192) */
 template <typename Dt_>
 struct PolicyRows {
   typedef Dt_ Dt;
   typedef typename Dt::raw raw;
-  const raw *logp, *old, *ref;      // old / ref may be NULL
+  const raw *logp, *old, *ref;      // old: logp itself where there is none (r = 1)
   long ld_logp, ld_old, ld_ref;
   const float* adv;
   long ld_adv;                      // 0: one per row
   Places pc;
   PolicyConst con;
   raw* dlogp;                       // NULL: no gradient
-  long ld_d, rows;
+  long ld_d;
+  int rows, gpr;                    // groups of a row
   float gscale;
-  int reduce;
 };
-struct PolicySums { double obj, kl, held, count; };
-// Groups of VEC places inside a row, numbered row by row; the thread takes g, g + step, ... and keeps (row, group of the row) by addition.  Groups in which
-// nothing counts read nothing.  weight(row, len) is the row's weight in the loss.
-template <typename Dt, typename W>
-__device__ __forceinline__ void policy_groups(const PolicyRows<Dt>& a, long g, long step, W&& weight, PolicySums& s) {
-  constexpr int V = Dt::VEC;
-  const long cols = a.pc.cols, gpr = (cols + V - 1) / V, drow = step / gpr, dcol = step - drow * gpr;
-  long row = g / gpr, col = g - row * gpr;
-  while (row < a.rows) {
-    const long c = col * V, left = cols - c, len = a.pc.len(row);
-    const unsigned in = a.pc.template bits<V>(row, c, len);
-    float out[V];
+// what a launch adds up: objective, KL (both weighted), places held by the clip, places
+enum { POLICY_OBJ, POLICY_KL, POLICY_HELD, POLICY_COUNT, POLICY_SUMS };
+struct PolicySums {
+  double obj, kl;
+  int held, count;
+  __device__ __forceinline__ PolicySums() : obj(0.0), kl(0.0), held(0), count(0) {}
+  __device__ __forceinline__ void to(double (&s)[POLICY_SUMS]) const { s[POLICY_OBJ] = obj; s[POLICY_KL] = kl; s[POLICY_HELD] = (double)held; s[POLICY_COUNT] = (double)count; }
+};
+// what a row's places share: length, weight in the loss, weight in the gradient, advantage (where it is one per row)
+struct PolicyRow { int len; double w; float wg; PolicySide side; };
+template <typename Dt>
+__device__ __forceinline__ PolicyRow policy_row(const PolicyRows<Dt>& a, int row, int len, double w) {
+  PolicyRow r;
+  r.len = len; r.w = w; r.wg = (float)(w * (double)a.gscale);
+  if (!a.ld_adv) r.side = PolicySide(a.con, a.adv[row]);
+  return r;
+}
+// The group of places c .. of a row.  A row's last group is moved back so that it ends with the row: every access is a whole one and no load stands in a branch
+// of its own, which would make the wave wait for one load before it issues the next; the places it shares with the group before are left out.  NARROW:
+// rows shorter than a group, read place by place (the last one in place of those outside).  A group in which nothing counts reads nothing.
+template <bool KL, bool NARROW, typename Dt>
+__device__ __forceinline__ void policy_group(const PolicyRows<Dt>& a, int row, int c, const PolicyRow& r, PolicySums& s) {
+  constexpr int V = POLICY_GROUP;
+  const int cols = (int)a.pc.cols, c0 = NARROW ? 0 : (c + V <= cols ? c : cols - V), skip = c - c0;
+  const unsigned in = (NARROW ? a.pc.template bits_end<V>(row, c0, r.len) : a.pc.template bits_inside<V>(row, c0, r.len)) >> skip << skip;
+  float out[V];
 #pragma unroll
-    for (int j = 0; j < V; j++) out[j] = 0.f;
-    if (in) {
-      float lp[V], old[V], ref[V], adv[V];
-      pcm_ld_group<Dt>(a.logp + row * a.ld_logp + c, left, lp);
-      if (a.old) pcm_ld_group<Dt>(a.old + row * a.ld_old + c, left, old);
-      if (a.ref) pcm_ld_group<Dt>(a.ref + row * a.ld_ref + c, left, ref);
-      if (a.ld_adv) pcm_ld_group<DtF32>(a.adv + row * a.ld_adv + c, left, adv);
-      else {
-        const float one = a.adv[row];
-#pragma unroll
-        for (int j = 0; j < V; j++) adv[j] = one;
-      }
-      const double w = weight(row, len);
-      const float wg = (float)(w * (double)a.gscale);
-      float so = 0.f, sk = 0.f;
-      int held = 0;
+  for (int j = 0; j < V; j++) out[j] = 0.f;
+  if (in) {
+    float lp[V], old[V], ref[V], adv[V];
+    const typename Dt::raw *pl = a.logp + at(row, a.ld_logp, c0), *po = a.old + at(row, a.ld_old, c0), *pr = KL ? a.ref + at(row, a.ld_ref, c0) : nullptr;
+    if constexpr (NARROW) {
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        float obj, kl, slope;
-        bool clipped;
-        policy_place(a.con, lp[j], a.old ? old[j] : lp[j], a.ref != nullptr, a.ref ? ref[j] : 0.f, adv[j], &obj, &kl, &slope, &clipped);
-        const bool counts = in >> j & 1u;
-        so += counts ? obj : 0.f;
-        sk += counts ? kl : 0.f;
-        held += counts && clipped ? 1 : 0;
-        out[j] = counts ? slope * wg : 0.f;
+        const int k = j < cols ? j : cols - 1;
+        lp[j] = Dt::ld(pl[k]); old[j] = Dt::ld(po[k]);
+        if (KL) ref[j] = Dt::ld(pr[k]);
       }
-      s.obj += w * (double)so; s.kl += w * (double)sk; s.held += (double)held; s.count += (double)__builtin_popcount(in);
+    } else {
+      pcm_ld_group<Dt, true>(pl, lp);
+      pcm_ld_group<Dt, true>(po, old);
+      if (KL) pcm_ld_group<Dt, true>(pr, ref);
     }
-    if (a.dlogp) pcm_st_group<Dt>(a.dlogp + row * a.ld_d + c, left, out);
-    col += dcol; row += drow;
-    if (col >= gpr) { col -= gpr; row++; }
+    PolicySide side = r.side;
+    if (a.ld_adv) {
+      const float* pa = a.adv + at(row, a.ld_adv, c0);
+      if constexpr (NARROW) {
+#pragma unroll
+        for (int j = 0; j < V; j++) adv[j] = pa[j < cols ? j : cols - 1];
+      } else {
+        pcm_ld_group<DtF32, true>(pa, adv);
+      }
+    }
+    float so = 0.f, sk = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      float obj, kl = 0.f, slope;
+      bool held;
+      if (a.ld_adv) side = PolicySide(a.con, adv[j]);
+      policy_place<KL>(a.con, side, lp[j], old[j], KL ? ref[j] : 0.f, &obj, &kl, &slope, &held);
+      const bool counts = in >> j & 1u;
+      so += counts ? obj : 0.f;
+      if (KL) sk += counts ? kl : 0.f;
+      s.held += counts && held ? 1 : 0;
+      out[j] = counts ? slope * r.wg : 0.f;
+    }
+    s.obj += r.w * (double)so;
+    if (KL) s.kl += r.w * (double)sk;
+    s.count += __builtin_popcount(in);
+  }
+  if (a.dlogp) {
+    typename Dt::raw* pd = a.dlogp + at(row, a.ld_d, c0);
+    if (!NARROW && skip == 0) pcm_st_group<Dt>(pd, V, out);
+    else
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (j >= skip && c0 + j < cols) pd[j] = Dt::st(out[j]);
   }
 }
-// how many places count, where the launch has to find out: per row (mean of row means) or in all, as partial sums over groups of 16 places
+// Groups numbered row by row; the thread takes g, g + NT, ... below end.  weight(row): the row's weight in the loss, asked for when the row changes
+template <bool KL, bool NARROW, int NT, typename Dt, typename W>
+__device__ __forceinline__ void policy_groups(const PolicyRows<Dt>& a, long g, long end, W&& weight, PolicySums& s) {
+  if (g >= end) return;
+  const int drow = NT / a.gpr, dcol = NT - drow * a.gpr;
+  int row = (int)(g / a.gpr), col = (int)(g - (long)row * a.gpr), last = -1;
+  PolicyRow r;
+  for (; g < end; g += NT) {
+    if (row != last) { last = row; r = policy_row(a, row, (int)a.pc.len(row), weight(row)); }
+    policy_group<KL, NARROW>(a, row, col * POLICY_GROUP, r, s);
+    col += dcol; row += drow;
+    if (col >= a.gpr) { col -= a.gpr; row++; }
+  }
+}
+// how many places count, where the launch has to find out, as partial sums over groups of 16 places
 __device__ __forceinline__ long count_groups(const Places& pc, long rows, long g, long step) {
   const long gpr = (pc.cols + 15) / 16, drow = step / gpr, dcol = step - drow * gpr;
   long row = g / gpr, col = g - row * gpr, n = 0;
@@ -422,90 +505,138 @@ __global__ __launch_bounds__(256) void policy_count_kernel(Places pc, long rows,
   n = pcm_block_sum<256>(n, red);
   if (threadIdx.x == 0) part[blockIdx.x] = (double)n;
 }
+// weights of rows, 1 / (places * rows): a wave to a row, or a workgroup where there are few long ones
 template <int TEAM>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void policy_count_rows_kernel(Places pc, long rows, double* count) {
-  __shared__ long red[16];
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void policy_weights_kernel(Places pc, long rows, double* weight) {
+  __shared__ int red[16];
   const long row = TEAM == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (row >= rows) return;
   const int tid = TEAM == 64 ? threadIdx.x & 63 : threadIdx.x;
   const long len = pc.len(row);
-  long n = 0;
-  for (long c = tid * 16L; c < len; c += TEAM * 16L) n += __builtin_popcount(pc.bits<16>(row, c, len));
-  n = pcm_block_sum<TEAM>(n, red);
-  if (tid == 0) count[row] = (double)n;
+  int n = 0;
+  if (pc.mask) {
+    for (long c = tid * 16L; c < len; c += TEAM * 16L) n += __builtin_popcount(pc.bits<16>(row, c, len));
+    n = pcm_block_sum<TEAM>(n, red);
+  } else n = (int)len;
+  if (tid == 0) weight[row] = 1.0 / (fmax((double)n, 1.0) * (double)rows);
 }
-// where the number of places comes from: the launch's arguments, partial sums of a launch before, or the lengths themselves
-struct PolicyCount { double known; const double* part; int nparts; const double* per_row; };
-template <typename Dt, int NT>
-__device__ __forceinline__ void policy_part(const PolicyRows<Dt>& a, const PolicyCount& pn, long g, long step, double* red, PolicySums& s) {
-  s.obj = s.kl = s.held = s.count = 0.0;
-  if (a.reduce == PCM_POLICY_TOKEN) {
-    double n = pn.known;
-    if (pn.part) {
-      n = 0.0;
-      for (int i = threadIdx.x; i < pn.nparts; i += NT) n += pn.part[i];
-      n = pcm_block_sum<NT>(n, red);
-    } else if (n < 0.0) {
-      long t = 0;
-      for (long r = threadIdx.x; r < a.rows; r += NT) t += a.pc.len(r);
-      n = pcm_block_sum<NT>((double)t, red);
-    }
-    const double w = 1.0 / fmax(n, 1.0);
-    policy_groups(a, g, step, [&](long, long) { return w; }, s);
-  } else if (a.reduce == PCM_POLICY_ROW) {
-    policy_groups(a, g, step, [&](long row, long len) { return 1.0 / ((pn.per_row ? pn.per_row[row] : (double)len) * (double)a.rows); }, s);
-  } else {
-    policy_groups(a, g, step, [&](long, long) { return 1.0; }, s);
+// sum of the lengths over a workgroup's threads, the loads of a thread independent of one another
+template <typename L>
+__device__ __forceinline__ long sum_lengths(const L* lengths, long rows, long cols, int nt) {
+  long t = 0;
+  for (long r = threadIdx.x; r < rows; r += 8L * nt) {
+    long v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = r + (long)u * nt < rows ? (long)lengths[r + (long)u * nt] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; u++) t += v[u] < 0 ? 0 : (v[u] > cols ? cols : v[u]);
   }
-  s.obj = pcm_block_sum<NT>(s.obj, red); s.kl = pcm_block_sum<NT>(s.kl, red);
-  s.held = pcm_block_sum<NT>(s.held, red); s.count = pcm_block_sum<NT>(s.count, red);
+  return t;
 }
-__device__ __forceinline__ void policy_result(const PolicySums& s, double kl, float* loss, float* stats) {
-  loss[0] = (float)(s.obj + kl * s.kl);
-  stats[0] = (float)s.obj; stats[1] = (float)s.kl; stats[2] = (float)(s.held / fmax(s.count, 1.0)); stats[3] = (float)s.count;
+// where the weights come from: one for all places -- 1 / places, the number of places being known (>= 0), the sum of `part`, or that of the lengths; or one
+// for each row
+struct PolicyWeight { double places; const double* part; int nparts; const double* per_row; };
+template <int NT>
+__device__ __forceinline__ double policy_weight(const Places& pc, int rows, const PolicyWeight& pw, double* red) {
+  double n = pw.places;
+  if (pw.part) {
+    n = 0.0;
+    for (int i = threadIdx.x; i < pw.nparts; i += NT) n += pw.part[i];
+    n = pcm_block_sum<NT>(n, red);
+  } else if (n < 0.0) {
+    n = (double)(pc.i64 ? sum_lengths((const int64_t*)pc.lengths, rows, pc.cols, NT) : sum_lengths((const int32_t*)pc.lengths, rows, pc.cols, NT));
+    n = pcm_block_sum<NT>(n, red);
+  }
+  return 1.0 / fmax(n, 1.0);
 }
-template <typename Dt>
-__global__ __launch_bounds__(256) void policy_main_kernel(PolicyRows<Dt> a, PolicyCount pn, double* part) {
-  __shared__ double red[4];
+template <bool KL, bool NARROW, int NT, typename Dt>
+__device__ __forceinline__ void policy_part(const PolicyRows<Dt>& a, const PolicyWeight& pw, long g, long end, double* red, double (&sum)[POLICY_SUMS]) {
   PolicySums s;
-  policy_part<Dt, 256>(a, pn, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, red, s);
-  if (threadIdx.x == 0) { double* q = part + 4 * (long)blockIdx.x; q[0] = s.obj; q[1] = s.kl; q[2] = s.held; q[3] = s.count; }
+  const double w = pw.per_row ? 0.0 : policy_weight<NT>(a.pc, a.rows, pw, red);
+  policy_groups<KL, NARROW, NT>(a, g, end, [&](int row) { return pw.per_row ? pw.per_row[row] : w; }, s);
+  s.to(sum);
+  pcm_block_sums<NT>(sum, red);
+}
+__device__ __forceinline__ void policy_result(const double (&s)[POLICY_SUMS], double kl, float* loss, float* stats) {
+  loss[0] = (float)(s[POLICY_OBJ] + kl * s[POLICY_KL]);
+  stats[0] = (float)s[POLICY_OBJ]; stats[1] = (float)s[POLICY_KL]; stats[2] = (float)(s[POLICY_HELD] / fmax(s[POLICY_COUNT], 1.0)); stats[3] = (float)s[POLICY_COUNT];
+}
+__device__ __forceinline__ void policy_store(const double (&s)[POLICY_SUMS], double* part) {
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int k = 0; k < POLICY_SUMS; k++) part[(long)blockIdx.x * POLICY_SUMS + k] = s[k];
+}
+// (256, 8): 8 waves to a SIMD, so that all 2048 workgroups are resident at once; a workgroup takes consecutive groups (a strided grid reads 15 % slower)
+template <bool KL, bool NARROW, typename Dt>
+__global__ __launch_bounds__(256, 8) void policy_main_kernel(PolicyRows<Dt> a, PolicyWeight pw, double* part) {
+  __shared__ double red[4 * POLICY_SUMS];
+  const long total = (long)a.rows * a.gpr, per = (total + gridDim.x - 1) / gridDim.x, g0 = blockIdx.x * per;
+  double s[POLICY_SUMS];
+  policy_part<KL, NARROW, 256>(a, pw, g0 + threadIdx.x, g0 + per < total ? g0 + per : total, red, s);
+  policy_store(s, part);
+}
+// the mean of row means, a row to a workgroup at a time: it counts the row's places first, and no launch has to do that before
+template <bool KL, typename Dt>
+__global__ __launch_bounds__(256, 8) void policy_row_kernel(PolicyRows<Dt> a, double* part) {
+  __shared__ double red[4 * POLICY_SUMS];
+  PolicySums t;
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int len = (int)a.pc.len(row);
+    int n = len;
+    if (a.pc.mask) {
+      n = 0;
+      for (int c = threadIdx.x * 16; c < len; c += 256 * 16) n += __builtin_popcount(a.pc.template bits<16>(row, c, len));
+      n = pcm_block_sum<256>(n, (int*)red);
+    }
+    const PolicyRow r = policy_row(a, row, len, 1.0 / (fmax((double)n, 1.0) * (double)a.rows));
+    for (int g = threadIdx.x; g < a.gpr; g += 256) policy_group<KL, false>(a, row, g * POLICY_GROUP, r, t);
+  }
+  double s[POLICY_SUMS];
+  t.to(s);
+  pcm_block_sums<256>(s, red);
+  policy_store(s, part);
 }
 __global__ __launch_bounds__(256) void policy_finish_kernel(const double* part, int nparts, double kl, float* loss, float* stats) {
-  __shared__ double red[4];
-  PolicySums s = {0.0, 0.0, 0.0, 0.0};
-  for (int i = threadIdx.x; i < nparts; i += 256) { s.obj += part[4 * i]; s.kl += part[4 * i + 1]; s.held += part[4 * i + 2]; s.count += part[4 * i + 3]; }
-  s.obj = pcm_block_sum<256>(s.obj, red); s.kl = pcm_block_sum<256>(s.kl, red);
-  s.held = pcm_block_sum<256>(s.held, red); s.count = pcm_block_sum<256>(s.count, red);
+  __shared__ double red[4 * POLICY_SUMS];
+  double s[POLICY_SUMS] = {0.0, 0.0, 0.0, 0.0};
+  for (int i = threadIdx.x; i < nparts; i += 256)
+#pragma unroll
+    for (int k = 0; k < POLICY_SUMS; k++) s[k] += part[i * POLICY_SUMS + k];
+  pcm_block_sums<256>(s, red);
   if (threadIdx.x == 0) policy_result(s, kl, loss, stats);
 }
 // few places: one workgroup counts, forms loss and gradient, and adds up, in one launch
 #define POLICY_SMALL_PLACES 16384
 #define POLICY_SMALL_ROWS 2048
-template <typename Dt>
-__global__ __launch_bounds__(1024) void policy_small_kernel(PolicyRows<Dt> a, double kl, float* loss, float* stats) {
-  __shared__ double red[16];
-  __shared__ double per_row[POLICY_SMALL_ROWS];
-  PolicyCount pn = {-1.0, nullptr, 0, nullptr};
-  if (a.pc.mask && a.reduce == PCM_POLICY_TOKEN) {
-    pn.known = pcm_block_sum<1024>((double)count_groups(a.pc, a.rows, threadIdx.x, 1024), red);
-  } else if (a.pc.mask && a.reduce == PCM_POLICY_ROW) {
-    for (long row = threadIdx.x >> 6; row < a.rows; row += 16) {
-      const long len = a.pc.len(row);
-      long n = 0;
-      for (long c = (threadIdx.x & 63) * 16L; c < len; c += 64 * 16L) n += __builtin_popcount(a.pc.template bits<16>(row, c, len));
-      n = pcm_lane_sum(n);
-      if ((threadIdx.x & 63) == 0) per_row[row] = (double)n;
+template <bool KL, bool NARROW, typename Dt>
+__global__ __launch_bounds__(1024) void policy_small_kernel(PolicyRows<Dt> a, int reduce, double kl, float* loss, float* stats) {
+  __shared__ double red[16 * POLICY_SUMS];
+  __shared__ double weight[POLICY_SMALL_ROWS];
+  PolicyWeight pw = {1.0, nullptr, 0, nullptr};
+  if (reduce == PCM_POLICY_TOKEN) {
+    if (a.pc.mask) pw.places = pcm_block_sum<1024>((double)count_groups(a.pc, a.rows, threadIdx.x, 1024), red);
+    else pw.places = a.pc.lengths ? -1.0 : (double)a.rows * (double)a.pc.cols;
+  } else if (reduce == PCM_POLICY_ROW) {
+    for (int row = threadIdx.x >> 6; row < a.rows; row += 16) {
+      const int len = (int)a.pc.len(row), lane = threadIdx.x & 63;
+      int n = len;
+      if (a.pc.mask) {
+        n = 0;
+        for (int c = lane * 16; c < len; c += 64 * 16) n += __builtin_popcount(a.pc.template bits<16>(row, c, len));
+        n = pcm_lane_sum(n);
+      }
+      if (lane == 0) weight[row] = 1.0 / (fmax((double)n, 1.0) * (double)a.rows);
     }
     __syncthreads();
-    pn.per_row = per_row;
+    pw.per_row = weight;
   }
-  PolicySums s;
-  policy_part<Dt, 1024>(a, pn, threadIdx.x, 1024, red, s);
+  double s[POLICY_SUMS];
+  policy_part<KL, NARROW, 1024>(a, pw, threadIdx.x, (long)a.rows * a.gpr, red, s);
   if (threadIdx.x == 0) policy_result(s, kl, loss, stats);
 }
 
 // ---- entry points ----
+#define AL_MAX_LD 4294967296L
 #define AL_MAX_ROWS 16777216L       /* 64 chunks of a row at the most: a grid stays below 2^31 workgroups */
 extern "C" size_t pcm_transition_logprob_workspace_bytes(long rows, long n) {
   if (rows <= 0 || n <= 0) return 0;
@@ -578,6 +709,8 @@ extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   if (rc != PCM_OK) return rc;
   PCM_CHECK(a->ld_logp >= a->cols && a->ld_ref >= a->cols && (!a->mask || a->ld_mask >= a->cols) && (!a->dlogp || a->ld_dlogp >= a->cols), PCM_EINVAL,
             "pcm_preference_loss: row stride below the row length");
+  PCM_CHECK(a->cols < AL_MAX_LD && a->ld_logp < AL_MAX_LD && a->ld_ref < AL_MAX_LD && a->ld_mask < AL_MAX_LD && a->ld_dlogp < AL_MAX_LD, PCM_EINVAL,
+            "pcm_preference_loss: row stride of 2^32 elements or more");
   PCM_CHECK(a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= pcm_preference_loss_workspace_bytes(a->pairs, a->cols), PCM_EINVAL,
             "pcm_preference_loss: workspace too small or not 8-byte aligned");
   const PairLoss pl = {a->beta, a->label_smoothing, a->kind};
@@ -591,53 +724,72 @@ extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   return pcm_post_launch("pcm_preference_loss");
 }
 static bool policy_small(long rows, long cols) { return rows <= POLICY_SMALL_ROWS && rows * cols <= POLICY_SMALL_PLACES; }
-static int policy_blocks(long rows, long cols, int vec) { return al_blocks(rows * ((cols + vec - 1) / vec)); }
+// a workgroup to a row: rows long enough to keep it busy, and enough of them for the chip or none too long for one
+static bool policy_by_row(int reduce, long rows, long cols) { return reduce == PCM_POLICY_ROW && cols >= 512 && (rows >= 512 || cols <= 4096); }
 #define POLICY_COUNT_PARTS 512
-extern "C" size_t pcm_policy_loss_workspace_bytes(long rows, long cols) {
+extern "C" size_t pcm_policy_loss_workspace_bytes(long rows, long cols) {      // partial counts or weights of rows, then the partial sums
   if (rows <= 0 || cols <= 0 || policy_small(rows, cols)) return 0;
-  return ((size_t)(rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS) + 4 * (size_t)policy_blocks(rows, cols, 4)) * sizeof(double);
+  return ((rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS) + POLICY_SUMS * 2048) * sizeof(double);
 }
+#define POLICY_LAUNCH(kernel, grid, block, ...)                                                                              \
+  do {                                                                                                                       \
+    if (a->cols < POLICY_GROUP) {                                                                                            \
+      if (kl) PCM_LAUNCH((kernel<true, true, Dt>), grid, block, 0, stream, __VA_ARGS__);                                     \
+      else PCM_LAUNCH((kernel<false, true, Dt>), grid, block, 0, stream, __VA_ARGS__);                                       \
+    } else if (kl) PCM_LAUNCH((kernel<true, false, Dt>), grid, block, 0, stream, __VA_ARGS__);                               \
+    else PCM_LAUNCH((kernel<false, false, Dt>), grid, block, 0, stream, __VA_ARGS__);                                        \
+  } while (0)
 extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
-  PCM_CHECK(a && a->logp && a->advantages && a->loss && a->stats && a->rows > 0 && a->rows <= AL_MAX_ROWS && a->cols > 0, PCM_EINVAL, "pcm_policy_loss: null/empty");
+  PCM_CHECK(a && a->logp && a->advantages && a->loss && a->stats && a->rows > 0 && a->rows <= AL_MAX_ROWS && a->cols > 0, PCM_EINVAL, "pcm_policy_loss: null/empty or too many rows");
   PCM_CHECK(pcm_dt_ok(a->dtype), PCM_EINVAL, "pcm_policy_loss: unknown element format %d", a->dtype);
   PCM_CHECK(a->reduce == PCM_POLICY_TOKEN || a->reduce == PCM_POLICY_ROW || a->reduce == PCM_POLICY_SUM, PCM_EINVAL, "pcm_policy_loss: unknown reduce %d", a->reduce);
   PCM_CHECK(a->clip_low >= 0.0 && a->clip_low < 1.0 && a->clip_high >= 0.0 && a->clip_high < 1e30, PCM_EINVAL, "pcm_policy_loss: clip_low must be in [0, 1), clip_high >= 0");
   PCM_CHECK(a->kl_coef == 0.0 || a->ref_logp, PCM_EINVAL, "pcm_policy_loss: a KL term needs the reference log-probabilities");
   PCM_CHECK(a->ld_logp >= a->cols && (!a->old_logp || a->ld_old >= a->cols) && (!a->ref_logp || a->ld_ref >= a->cols) && (a->adv_per_row || a->ld_adv >= a->cols) &&
                 (!a->mask || a->ld_mask >= a->cols) && (!a->dlogp || a->ld_dlogp >= a->cols), PCM_EINVAL, "pcm_policy_loss: row stride below the row length");
+  PCM_CHECK(a->cols < 2147483648L - 65536 && a->ld_logp < AL_MAX_LD && a->ld_old < AL_MAX_LD && a->ld_ref < AL_MAX_LD && a->ld_adv < AL_MAX_LD && a->ld_mask < AL_MAX_LD &&
+                a->ld_dlogp < AL_MAX_LD, PCM_EINVAL, "pcm_policy_loss: row stride of 2^32 elements or more");
   const size_t need = pcm_policy_loss_workspace_bytes(a->rows, a->cols);
   PCM_CHECK(need == 0 || (a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= need), PCM_EINVAL,
             "pcm_policy_loss: workspace too small or not 8-byte aligned");
   const Places pc = {a->mask, a->ld_mask, a->lengths, a->lengths_i64, a->cols};
-  const PolicyConst con = {log1p(a->clip_high), log1p(-a->clip_low), (float)(1.0 + a->clip_high), (float)(1.0 - a->clip_low), (float)a->kl_coef};
+  const PolicyConst con = {log1p(a->clip_high), log1p(-a->clip_low), (float)log1p(a->clip_high), (float)log1p(-a->clip_low), (float)(1.0 + a->clip_high), (float)(1.0 - a->clip_low), (float)a->kl_coef};
   const long rows = a->rows;
   const int reduce = a->reduce == PCM_POLICY_ROW && rows == 1 ? PCM_POLICY_TOKEN : a->reduce;      // one row: its mean is the mean of all places
+  const bool kl = a->ref_logp != nullptr, by_row = policy_by_row(reduce, rows, a->cols);
+  const int gpr = (int)((a->cols + POLICY_GROUP - 1) / POLICY_GROUP);
   pcm_with_dtype(a->dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    const PolicyRows<Dt> r = {(cp)a->logp, (cp)a->old_logp, (cp)a->ref_logp, a->ld_logp, a->ld_old, a->ld_ref, a->advantages, a->adv_per_row ? 0 : a->ld_adv, pc, con,
-                              (typename Dt::raw*)a->dlogp, a->ld_dlogp, rows, (float)a->grad_scale, reduce};
+    const PolicyRows<Dt> r = {(cp)a->logp, (cp)(a->old_logp ? a->old_logp : a->logp), (cp)a->ref_logp, a->ld_logp, a->old_logp ? a->ld_old : a->ld_logp, a->ld_ref,
+                              a->advantages, a->adv_per_row ? 0 : a->ld_adv, pc, con, (typename Dt::raw*)a->dlogp, a->ld_dlogp, (int)rows, gpr, (float)a->grad_scale};
     if (need == 0) {
-      PCM_LAUNCH(policy_small_kernel<Dt>, dim3(1), dim3(1024), 0, stream, r, a->kl_coef, a->loss, a->stats);
+      POLICY_LAUNCH(policy_small_kernel, dim3(1), dim3(1024), r, reduce, a->kl_coef, a->loss, a->stats);
       return;
     }
     double *counts = (double*)a->workspace, *part = counts + (rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS);
-    PolicyCount pn = {-1.0, nullptr, 0, nullptr};
-    if (reduce == PCM_POLICY_TOKEN) {
-      if (!a->mask && !a->lengths) pn.known = (double)rows * (double)a->cols;
-      else if (a->mask || rows > 4096) {          // (up to 4096 lengths each workgroup adds up itself: 16 loads a thread against a launch)
-        const long b = a->mask ? al_blocks(rows * ((a->cols + 15) / 16)) : al_blocks(rows);
-        pn.nparts = (int)(b < POLICY_COUNT_PARTS ? b : POLICY_COUNT_PARTS);
-        pn.part = counts;
-        PCM_LAUNCH(policy_count_kernel, dim3(pn.nparts), dim3(256), 0, stream, pc, rows, counts);
+    int nb = al_blocks(rows * gpr);
+    if (by_row) {
+      nb = (int)(rows < PCM_GRID_CAP(2048) ? rows : PCM_GRID_CAP(2048));
+      if (kl) PCM_LAUNCH((policy_row_kernel<true, Dt>), dim3(nb), dim3(256), 0, stream, r, part);
+      else PCM_LAUNCH((policy_row_kernel<false, Dt>), dim3(nb), dim3(256), 0, stream, r, part);
+    } else {
+      PolicyWeight pw = {1.0, nullptr, 0, nullptr};
+      if (reduce == PCM_POLICY_TOKEN) {
+        pw.places = a->mask || a->lengths ? -1.0 : (double)rows * (double)a->cols;
+        if (a->mask || (a->lengths && rows > 4096)) {      // (up to 4096 lengths each workgroup adds up itself: 16 loads a thread against a launch)
+          const long b = a->mask ? al_blocks(rows * ((a->cols + 15) / 16)) : al_blocks(rows);
+          pw.nparts = (int)(b < POLICY_COUNT_PARTS ? b : POLICY_COUNT_PARTS);
+          pw.part = counts;
+          PCM_LAUNCH(policy_count_kernel, dim3(pw.nparts), dim3(256), 0, stream, pc, rows, counts);
+        }
+      } else if (reduce == PCM_POLICY_ROW) {
+        pw.per_row = counts;
+        if (a->cols <= 4096) PCM_LAUNCH(policy_weights_kernel<64>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, pc, rows, counts);
+        else PCM_LAUNCH(policy_weights_kernel<1024>, dim3((unsigned)rows), dim3(1024), 0, stream, pc, rows, counts);
       }
-    } else if (reduce == PCM_POLICY_ROW && a->mask) {
-      pn.per_row = counts;
-      if (a->cols <= 4096) PCM_LAUNCH(policy_count_rows_kernel<64>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, pc, rows, counts);
-      else PCM_LAUNCH(policy_count_rows_kernel<1024>, dim3((unsigned)rows), dim3(1024), 0, stream, pc, rows, counts);
+      POLICY_LAUNCH(policy_main_kernel, dim3(nb), dim3(256), r, pw, part);
     }
-    const int nb = policy_blocks(rows, a->cols, Dt::VEC);
-    PCM_LAUNCH(policy_main_kernel<Dt>, dim3(nb), dim3(256), 0, stream, r, pn, part);
     PCM_LAUNCH(policy_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)part, nb, a->kl_coef, a->loss, a->stats);
   });
   return pcm_post_launch("pcm_policy_loss");
