@@ -550,7 +550,8 @@ int pcm_policy_loss(const pcm_policy_args* a, void* stream);
  * `chunks` is a table in DEVICE memory: the tensors cut into pieces of n <= PCM_GRAD_CHUNK consecutive elements, `total` elements in all.
  * dst may be src (then nothing is written when nothing has to be clipped) or a place apart; its format may be another one.  Pieces that are
  * written must not overlap one another or any other piece that is read.  sumsq is what pcm_adamw_clip_step takes as gradsq. */
-#define PCM_GRAD_CHUNK 16384
+#define PCM_GRAD_CHUNK 8192
+#define PCM_GRAD_CHUNK_SMALL 1024 /* for up to 32768 elements in all: up to 64 such pieces take one launch instead of two */
 typedef struct {
   const void* src;
   void* dst;

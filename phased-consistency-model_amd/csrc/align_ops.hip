@@ -8,9 +8,11 @@
 
 static inline int al_blocks(long n) { long b = (n + 255) / 256; return (int)(b > PCM_GRID_CAP(2048) ? PCM_GRID_CAP(2048) : (b < 1 ? 1 : b)); }
 
+#define AL_U (16 / Dt::VEC)      /* groups of a thread in flight: 16 elements of every tensor */
 // how a launch cuts rows of n elements: teams of 64 (four rows to a workgroup) for short rows, else `chunks` workgroups of 256 per row, so that some
 // 4096 workgroups (two rounds of 8 per CU) share the work; at most 64 chunks, whose partial sums one wave adds up with one load per lane.
 struct RowCut { int team, chunks; long len; };
+#define ROW_TEAM_MAX 65536L
 static RowCut row_cut(long rows, long n, int vec) {
   RowCut c = {256, 1, n};
   if (n <= 1024) { c.team = 64; return c; }
@@ -25,6 +27,7 @@ static inline unsigned row_cut_blocks(const RowCut& c, long rows) { return (unsi
 // (row, chunk, thread of the team) of a thread; false: a team past the last row
 template <int TEAM>
 __device__ __forceinline__ bool row_cut_place(long block, long rows, int chunks, long* row, int* chunk, int* tid) {
+  if (TEAM == 1024) { *row = block; *chunk = 0; *tid = threadIdx.x; return true; }
   if (TEAM == 64) { *row = block * 4 + (threadIdx.x >> 6); *chunk = 0; *tid = threadIdx.x & 63; return *row < rows; }
   *row = block / chunks; *chunk = (int)(block - *row * chunks); *tid = threadIdx.x;
   return true;
@@ -37,16 +40,16 @@ __device__ __forceinline__ float transition_value(double acc, double s, long n, 
   return (float)(mean_reduce ? per : per * (double)n);
 }
 template <typename Dt, int TEAM>
-__global__ __launch_bounds__(256) void transition_fwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std, float* logp, double* part,
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void transition_fwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std, float* logp, double* part,
                                                              long rows, long n, int chunks, long len, int mean_reduce) {
-  __shared__ double red[4];
+  __shared__ double red[16];
   long row; int chunk, tid;
   if (!row_cut_place<TEAM>(blockIdx.x, rows, chunks, &row, &chunk, &tid)) return;
   const long i0 = chunk * len, i1 = i0 + len < n ? i0 + len : n;
   const typename Dt::raw *xr = x + row * n, *mr = mean + row * n;
-  float a[4][Dt::VEC], b[4][Dt::VEC];
+  float a[AL_U][Dt::VEC], b[AL_U][Dt::VEC];
   double acc = 0.0;
-  pcm_groups<Dt, TEAM, 4>(i0, i1, tid,
+  pcm_groups<Dt, TEAM, AL_U>(i0, i1, tid,
     [&](int u, long i, long left) { pcm_ld_group<Dt>(xr + i, left, a[u]); pcm_ld_group<Dt>(mr + i, left, b[u]); },
     [&](int u, long i, long left) {
       float t = 0.f;
@@ -77,8 +80,8 @@ __global__ __launch_bounds__(256) void transition_bwd_kernel(const typename Dt::
   typename Dt::raw* dr = dmean + row * n;
   const double s = (double)std[row];
   const float f = (float)((double)dlogp[row] / (s * s * (mean_reduce ? (double)n : 1.0)));
-  float a[4][Dt::VEC], b[4][Dt::VEC];
-  pcm_groups<Dt, TEAM, 4>(i0, i1, tid,
+  float a[AL_U][Dt::VEC], b[AL_U][Dt::VEC];
+  pcm_groups<Dt, TEAM, AL_U>(i0, i1, tid,
     [&](int u, long i, long left) { pcm_ld_group<Dt>(xr + i, left, a[u]); pcm_ld_group<Dt>(mr + i, left, b[u]); },
     [&](int u, long i, long left) {
 #pragma unroll
@@ -122,9 +125,9 @@ struct DenoiseRows {
   template <int NT>
   __device__ __forceinline__ void sums(long row, long i0, long i1, int tid, double (&acc)[SUMS]) const {
     const long o = row * n;
-    float t[4][Dt::VEC], p[4][Dt::VEC], r[4][Dt::VEC];
+    float t[AL_U][Dt::VEC], p[AL_U][Dt::VEC], r[AL_U][Dt::VEC];
     double s = 0.0;
-    pcm_groups<Dt, NT, 4>(i0, i1, tid,
+    pcm_groups<Dt, NT, AL_U>(i0, i1, tid,
       [&](int u, long i, long left) {
         pcm_ld_group<Dt, true>(target + o + i, left, t[u]); pcm_ld_group<Dt, true>(pred + o + i, left, p[u]); pcm_ld_group<Dt, true>(ref + o + i, left, r[u]);
       },
@@ -139,8 +142,8 @@ struct DenoiseRows {
   template <int NT>
   __device__ __forceinline__ void grad(long row, long i0, long i1, int tid, float f) const {
     const long o = row * n;
-    float t[4][Dt::VEC], p[4][Dt::VEC];
-    pcm_groups<Dt, NT, 4>(i0, i1, tid,
+    float t[AL_U][Dt::VEC], p[AL_U][Dt::VEC];
+    pcm_groups<Dt, NT, AL_U>(i0, i1, tid,
       [&](int u, long i, long left) { pcm_ld_group<Dt, true>(target + o + i, left, t[u]); pcm_ld_group<Dt, true>(pred + o + i, left, p[u]); },
       [&](int u, long i, long left) {
 #pragma unroll
@@ -306,11 +309,51 @@ __global__ __launch_bounds__(256) void pair_grad_kernel(R rows_, const double* p
   const double f = (row < pairs ? s * rows_.factor(row, up) : -s * rows_.factor(row, down)) * gscale / (double)pairs;
   rows_.template grad<TEAM>(row, i0, i1, tid, (float)f);
 }
+// few elements: one workgroup takes all pairs in one launch -- a row to a wave, or to all waves where rows are long
+#define PAIR_SMALL_ELEMENTS 32768L
+#define PAIR_SMALL_ROWS 128
+template <typename R>
+__global__ __launch_bounds__(1024) void pair_small_kernel(R rows_, PairLoss pl, double gscale, float* loss, float* log_ratio, int pairs, int n, int want_grad) {
+  __shared__ double red[16], rho[PAIR_SMALL_ROWS], factor[PAIR_SMALL_ROWS], slope[PAIR_SMALL_ROWS / 2];
+  const int rows = 2 * pairs, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const bool by_wave = n <= 1024;
+  double s[R::SUMS];
+  for (int row = by_wave ? wave : 0; row < rows; row += by_wave ? 16 : 1) {
+    if (by_wave) rows_.template sums<64>(row, 0, n, lane, s);
+    else rows_.template sums<1024>(row, 0, n, threadIdx.x, s);
+#pragma unroll
+    for (int a = 0; a < R::SUMS; a++) s[a] = by_wave ? pcm_lane_sum(s[a]) : pcm_block_sum<1024>(s[a], red);
+    if (by_wave ? lane == 0 : threadIdx.x == 0) {
+      rho[row] = rows_.rho(row, s); factor[row] = rows_.factor(row, s);
+      log_ratio[row] = (float)rho[row];
+    }
+  }
+  __syncthreads();
+  double l = 0.0;
+  if ((int)threadIdx.x < pairs) pair_loss(pl, rho[threadIdx.x] - rho[pairs + threadIdx.x], &l, &slope[threadIdx.x]);
+  l = pcm_block_sum<1024>(l, red);
+  if (threadIdx.x == 0) loss[0] = (float)(l / (double)pairs);
+  if (!want_grad) return;
+  for (int row = by_wave ? wave : 0; row < rows; row += by_wave ? 16 : 1) {
+    const float f = (float)((row < pairs ? slope[row] : -slope[row - pairs]) * factor[row] * gscale / (double)pairs);
+    if (by_wave) rows_.template grad<64>(row, 0, n, lane, f);
+    else rows_.template grad<1024>(row, 0, n, threadIdx.x, f);
+  }
+}
+static bool pair_small(long rows, long n) { return rows <= PAIR_SMALL_ROWS && rows * n <= PAIR_SMALL_ELEMENTS; }
 // bytes of the partial sums
-static size_t pair_ws_bytes(long rows, long n, int vec, int sums) { const RowCut c = row_cut(rows, n, vec); return (size_t)rows * c.chunks * sums * sizeof(double); }
+static size_t pair_ws_bytes(long rows, long n, int sums) {      // (the 16-bit formats cut into no more chunks than fp32)
+  if (pair_small(rows, n)) return 0;
+  const RowCut c = row_cut(rows, n, 4);
+  return (size_t)rows * c.chunks * sums * sizeof(double);
+}
 template <typename R>
 static void pair_launch(const R& r, double* part, const PairLoss& pl, double gscale, float* loss, float* log_ratio, long pairs, long n, void* stream) {
   const long rows = 2 * pairs;
+  if (pair_small(rows, n)) {
+    PCM_LAUNCH(pair_small_kernel<R>, dim3(1), dim3(1024), 0, stream, r, pl, gscale, loss, log_ratio, (int)pairs, (int)n, r.wants_grad() ? 1 : 0);
+    return;
+  }
   const RowCut c = row_cut(rows, n, R::Dt::VEC);
   const unsigned nb = row_cut_blocks(c, rows), ng = r.wants_grad() ? nb + 1 : 1;
   if (c.team == 64) {
@@ -638,16 +681,18 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(PolicyRows<Dt> a, in
 // ---- entry points ----
 #define AL_MAX_LD 4294967296L
 #define AL_MAX_ROWS 16777216L       /* 64 chunks of a row at the most: a grid stays below 2^31 workgroups */
+// the forward pass takes a row to a workgroup of 1024 where rows are too few for one chunk each but short enough: one launch instead of two, 16 rows of
+// 16384 in 2.3 us against 3.1 + 2.5
+static RowCut transition_cut(long rows, long n, int vec) {
+  RowCut c = row_cut(rows, n, vec);
+  if (c.chunks > 1 && n <= ROW_TEAM_MAX) { c.team = 1024; c.chunks = 1; c.len = n; }
+  return c;
+}
 extern "C" size_t pcm_transition_logprob_workspace_bytes(long rows, long n) {
   if (rows <= 0 || n <= 0) return 0;
-  const RowCut c = row_cut(rows, n, 4);      // (the 16-bit formats cut into no more chunks than fp32)
+  const RowCut c = transition_cut(rows, n, 4);      // (the 16-bit formats cut into no more chunks than fp32)
   return c.chunks > 1 ? (size_t)rows * c.chunks * sizeof(double) : 0;
 }
-#define TRANSITION_LAUNCH(kernel, ...)                                                                                       \
-  do {                                                                                                                       \
-    if (c.team == 64) PCM_LAUNCH((kernel<Dt, 64>), dim3(row_cut_blocks(c, rows)), dim3(256), 0, stream, __VA_ARGS__);        \
-    else PCM_LAUNCH((kernel<Dt, 256>), dim3(row_cut_blocks(c, rows)), dim3(256), 0, stream, __VA_ARGS__);                    \
-  } while (0)
 extern "C" int pcm_transition_logprob(const void* x, const void* mean, const float* std, int dtype, int mean_reduce, float* logp, long rows, long n,
                                       void* workspace, size_t workspace_bytes, void* stream) {
   PCM_CHECK(x && mean && std && logp && pcm_dt_ok(dtype) && rows > 0 && rows <= AL_MAX_ROWS && n > 0, PCM_EINVAL, "pcm_transition_logprob: null/empty or unknown format");
@@ -657,8 +702,12 @@ extern "C" int pcm_transition_logprob(const void* x, const void* mean, const flo
   pcm_with_dtype(dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
-    const RowCut c = row_cut(rows, n, Dt::VEC);
-    TRANSITION_LAUNCH(transition_fwd_kernel, (cp)x, (cp)mean, std, logp, (double*)workspace, rows, n, c.chunks, c.len, mean_reduce);
+    const RowCut c = transition_cut(rows, n, Dt::VEC);
+    const dim3 grid(c.team == 1024 ? (unsigned)rows : row_cut_blocks(c, rows));
+    double* part = (double*)workspace;
+    if (c.team == 64) PCM_LAUNCH((transition_fwd_kernel<Dt, 64>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, logp, part, rows, n, c.chunks, c.len, mean_reduce);
+    else if (c.team == 256) PCM_LAUNCH((transition_fwd_kernel<Dt, 256>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, logp, part, rows, n, c.chunks, c.len, mean_reduce);
+    else PCM_LAUNCH((transition_fwd_kernel<Dt, 1024>), grid, dim3(1024), 0, stream, (cp)x, (cp)mean, std, logp, part, rows, n, c.chunks, c.len, mean_reduce);
     if (c.chunks > 1)
       PCM_LAUNCH(transition_finish_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, (const double*)workspace, std, logp, rows, n, c.chunks, mean_reduce);
   });
@@ -672,7 +721,9 @@ extern "C" int pcm_transition_logprob_bwd(const void* x, const void* mean, const
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
     const RowCut c = row_cut(rows, n, Dt::VEC);
-    TRANSITION_LAUNCH(transition_bwd_kernel, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, c.chunks, c.len, mean_reduce);
+    const dim3 grid(row_cut_blocks(c, rows));
+    if (c.team == 64) PCM_LAUNCH((transition_bwd_kernel<Dt, 64>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, c.chunks, c.len, mean_reduce);
+    else PCM_LAUNCH((transition_bwd_kernel<Dt, 256>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, c.chunks, c.len, mean_reduce);
   });
   return pcm_post_launch("pcm_transition_logprob_bwd");
 }
@@ -685,12 +736,13 @@ static int pair_args_ok(const char* who, int dtype, long pairs, double beta, int
   PCM_CHECK(eps >= 0.0 && eps < 0.5 && (eps == 0.0 || kind == PCM_PAIR_SIGMOID), PCM_EINVAL, "%s: label smoothing must be in [0, 0.5) and needs the sigmoid kind", who);
   return PCM_OK;
 }
-extern "C" size_t pcm_denoise_preference_loss_workspace_bytes(long pairs, long n) { return pairs > 0 && n > 0 ? pair_ws_bytes(2 * pairs, n, 4, DenoiseRows<DtF32>::SUMS) : 0; }
+extern "C" size_t pcm_denoise_preference_loss_workspace_bytes(long pairs, long n) { return pairs > 0 && n > 0 ? pair_ws_bytes(2 * pairs, n, DenoiseRows<DtF32>::SUMS) : 0; }
 extern "C" int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a, void* stream) {
   PCM_CHECK(a && a->pred && a->ref && a->target && a->loss && a->log_ratio && a->n > 0, PCM_EINVAL, "pcm_denoise_preference_loss: null/empty");
   const int rc = pair_args_ok("pcm_denoise_preference_loss", a->dtype, a->pairs, a->beta, a->kind, a->label_smoothing);
   if (rc != PCM_OK) return rc;
-  PCM_CHECK(a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= pcm_denoise_preference_loss_workspace_bytes(a->pairs, a->n), PCM_EINVAL,
+  const size_t need = pcm_denoise_preference_loss_workspace_bytes(a->pairs, a->n);
+  PCM_CHECK(need == 0 || (a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= need), PCM_EINVAL,
             "pcm_denoise_preference_loss: workspace too small or not 8-byte aligned");
   const PairLoss pl = {a->beta, a->label_smoothing, a->kind};
   const double k = a->mean_reduce ? 1.0 / (double)a->n : 1.0;
@@ -702,7 +754,7 @@ extern "C" int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a,
   });
   return pcm_post_launch("pcm_denoise_preference_loss");
 }
-extern "C" size_t pcm_preference_loss_workspace_bytes(long pairs, long cols) { return pairs > 0 && cols > 0 ? pair_ws_bytes(2 * pairs, cols, 4, TokenRows<DtF32>::SUMS) : 0; }
+extern "C" size_t pcm_preference_loss_workspace_bytes(long pairs, long cols) { return pairs > 0 && cols > 0 ? pair_ws_bytes(2 * pairs, cols, TokenRows<DtF32>::SUMS) : 0; }
 extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   PCM_CHECK(a && a->logp && a->ref_logp && a->loss && a->log_ratio && a->cols > 0, PCM_EINVAL, "pcm_preference_loss: null/empty");
   const int rc = pair_args_ok("pcm_preference_loss", a->dtype, a->pairs, a->beta, a->kind, a->label_smoothing);
@@ -711,7 +763,8 @@ extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
             "pcm_preference_loss: row stride below the row length");
   PCM_CHECK(a->cols < AL_MAX_LD && a->ld_logp < AL_MAX_LD && a->ld_ref < AL_MAX_LD && a->ld_mask < AL_MAX_LD && a->ld_dlogp < AL_MAX_LD, PCM_EINVAL,
             "pcm_preference_loss: row stride of 2^32 elements or more");
-  PCM_CHECK(a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= pcm_preference_loss_workspace_bytes(a->pairs, a->cols), PCM_EINVAL,
+  const size_t need = pcm_preference_loss_workspace_bytes(a->pairs, a->cols);
+  PCM_CHECK(need == 0 || (a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= need), PCM_EINVAL,
             "pcm_preference_loss: workspace too small or not 8-byte aligned");
   const PairLoss pl = {a->beta, a->label_smoothing, a->kind};
   const Places pc = {a->mask, a->ld_mask, a->lengths, a->lengths_i64, a->cols};

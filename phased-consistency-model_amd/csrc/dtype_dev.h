@@ -61,14 +61,15 @@ __device__ __forceinline__ void pcm_ld_group(const typename Dt::raw* p, long lef
 #pragma unroll
   for (int j = 0; j < N; j++) v[j] = j < left ? Dt::ld(p[j]) : 0.f;
 }
-template <typename Dt, int N>
+template <typename Dt, bool NT = false, int N>
 __device__ __forceinline__ void pcm_st_group(typename Dt::raw* p, long left, const float (&v)[N]) {
   if (left >= N) {
     typedef typename Dt::raw vec __attribute__((ext_vector_type(N), aligned(sizeof(typename Dt::raw))));
     vec r;
 #pragma unroll
     for (int j = 0; j < N; j++) r[j] = Dt::st(v[j]);
-    *(vec*)p = r;
+    if (NT) __builtin_nontemporal_store(r, (vec*)p);
+    else *(vec*)p = r;
     return;
   }
 #pragma unroll

@@ -10,7 +10,7 @@ __device__ __forceinline__ double piece_sumsq(const void* src, int n, int tid) {
   const typename Dt::raw* p = (const typename Dt::raw*)src;
   float v[4][Dt::VEC];
   double acc = 0.0;
-  pcm_groups<Dt, NT, 4>(0, n, tid, [&](int u, long i, long left) { pcm_ld_group<Dt>(p + i, left, v[u]); },
+  pcm_groups<Dt, NT, 4>(0, n, tid, [&](int u, long i, long left) { pcm_ld_group<Dt, true>(p + i, left, v[u]); },
     [&](int u, long i, long left) {
 #pragma unroll
       for (int j = 0; j < Dt::VEC; j++) acc += (double)v[u][j] * (double)v[u][j];
@@ -24,11 +24,11 @@ __device__ __forceinline__ void piece_scale(const void* src, void* dst, float f,
   const typename S::raw* p = (const typename S::raw*)src;
   typename D::raw* q = (typename D::raw*)dst;
   float v[4][N];
-  pcm_groups<W, NT, 4>(0, n, tid, [&](int u, long i, long left) { pcm_ld_group<S>(p + i, left, v[u]); },
+  pcm_groups<W, NT, 4>(0, n, tid, [&](int u, long i, long left) { pcm_ld_group<S, true>(p + i, left, v[u]); },
     [&](int u, long i, long left) {
 #pragma unroll
       for (int j = 0; j < N; j++) v[u][j] *= f;
-      pcm_st_group<D>(q + i, left, v[u]);
+      pcm_st_group<D, true>(q + i, left, v[u]);
     });
 }
 template <int NT>
@@ -71,40 +71,41 @@ __global__ __launch_bounds__(256) void grad_norm_finish_kernel(const double* par
   const double t = grad_total(part, n, red);
   if (threadIdx.x == 0) { sumsq[0] = t; norm[0] = (float)sqrt(t); }
 }
-// every workgroup adds up the partial sums again (16 KB out of L2) instead of waiting for a launch that does it once; the pieces are taken last to
-// first, so that those the sum has read last, which are still in the 256 MB cache behind L2, come first
+// Every workgroup adds up the partial sums again (8 KB out of L2) instead of waiting for a launch that does it once.  At 285 MB in and out: a piece to a
+// workgroup 155 us against 162 with 4096 workgroups (the sum: 1024 are as fast as 4096, and fewer partial sums), nontemporal stores 147.
 __global__ __launch_bounds__(256) void grad_scale_kernel(const pcm_grad_chunk* chunks, int nchunks, const double* part, int nparts, double max_norm, float* norm,
                                                          double* sumsq) {
   __shared__ double red[4];
   const double t = grad_total(part, nparts, red);
   if (blockIdx.x == 0 && threadIdx.x == 0) { sumsq[0] = t; norm[0] = (float)sqrt(t); }
   const float f = clip_factor(t, max_norm);
-  for (int c = nchunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) chunk_scale<256>(chunks[c], f, threadIdx.x);
+  for (int c = (int)blockIdx.x; c < nchunks; c += gridDim.x) chunk_scale<256>(chunks[c], f, threadIdx.x);
 }
-// few elements: one workgroup does it all in one launch, four teams of 256 taking pieces in turn (max_norm <= 0: the norm alone).  The pieces' records
-// are read once, into LDS, so that a piece waits for its data only.
-#define GRAD_SMALL_CHUNKS 256
+// few elements in few pieces: one workgroup does it all in one launch, its 16 waves taking pieces in turn (max_norm <= 0: the norm alone).  The pieces'
+// records are read once, into LDS, so that a piece waits for its data only.
+#define GRAD_SMALL_CHUNKS 64
 __global__ __launch_bounds__(1024) void grad_small_kernel(const pcm_grad_chunk* chunks, int nchunks, double max_norm, float* norm, double* sumsq) {
   __shared__ pcm_grad_chunk tab[GRAD_SMALL_CHUNKS];
   __shared__ double red[16];
   if ((int)threadIdx.x < nchunks) tab[threadIdx.x] = chunks[threadIdx.x];
   __syncthreads();
-  const int team = threadIdx.x >> 8, tid = threadIdx.x & 255;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   double acc = 0.0;
-  for (int c = team; c < nchunks; c += 4) acc += chunk_sumsq<256>(tab[c], tid);
+  for (int c = wave; c < nchunks; c += 16) acc += chunk_sumsq<64>(tab[c], lane);
   acc = pcm_block_sum<1024>(acc, red);
   if (threadIdx.x == 0) { sumsq[0] = acc; norm[0] = (float)sqrt(acc); }
   if (max_norm > 0.0) {
     const float f = clip_factor(acc, max_norm);
-    for (int c = team; c < nchunks; c += 4) chunk_scale<256>(tab[c], f, tid);
+    for (int c = wave; c < nchunks; c += 16) chunk_scale<64>(tab[c], f, lane);
   }
 }
-// One workgroup against two launches: the second launch costs about 4 us, a workgroup alone moves some 60 KB a microsecond.
+// One workgroup against two launches: the second launch costs about 4 us, a round of 16 pieces of 1024 elements about 1 us each way.
 #define GRAD_SMALL_ELEMENTS 32768
 static bool grad_small(int nchunks, long total) { return total <= GRAD_SMALL_ELEMENTS && nchunks <= GRAD_SMALL_CHUNKS; }
-static int grad_blocks(int nchunks) { const int cap = PCM_GRID_CAP(2048); return nchunks < cap ? nchunks : cap; }
+static int grad_blocks(int nchunks, int cap) { return nchunks < cap ? nchunks : cap; }
+#define GRAD_PARTS PCM_GRID_CAP(1024)
 extern "C" size_t pcm_grad_norm_workspace_bytes(int nchunks, long total) {
-  return nchunks > 0 && !grad_small(nchunks, total) ? (size_t)grad_blocks(nchunks) * sizeof(double) : 0;
+  return nchunks > 0 && !grad_small(nchunks, total) ? (size_t)grad_blocks(nchunks, GRAD_PARTS) * sizeof(double) : 0;
 }
 static int grad_run(const char* who, const pcm_grad_chunk* chunks, int nchunks, long total, double max_norm, float* norm, double* sumsq, void* workspace,
                     size_t workspace_bytes, void* stream) {
@@ -116,10 +117,10 @@ static int grad_run(const char* who, const pcm_grad_chunk* chunks, int nchunks, 
     PCM_LAUNCH(grad_small_kernel, dim3(1), dim3(1024), 0, stream, chunks, nchunks, max_norm, norm, sumsq);
     return pcm_post_launch(who);
   }
-  const int nb = grad_blocks(nchunks);
+  const int nb = grad_blocks(nchunks, GRAD_PARTS);
   PCM_LAUNCH(grad_sumsq_kernel, dim3(nb), dim3(256), 0, stream, chunks, nchunks, (double*)workspace);
   if (max_norm > 0.0)
-    PCM_LAUNCH(grad_scale_kernel, dim3(nb), dim3(256), 0, stream, chunks, nchunks, (const double*)workspace, nb, max_norm, norm, sumsq);
+    PCM_LAUNCH(grad_scale_kernel, dim3(grad_blocks(nchunks, PCM_GRID_CAP(16384))), dim3(256), 0, stream, chunks, nchunks, (const double*)workspace, nb, max_norm, norm, sumsq);
   else
     PCM_LAUNCH(grad_norm_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)workspace, nb, norm, sumsq);
   return pcm_post_launch(who);

@@ -26,7 +26,7 @@ SRC_DIRECT, SRC_UPSAMPLE2, SRC_ZEROINS2 = 0, 1, 2
 DT_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # PCM_DT_*: element formats named per call (alignment operators)
 PAIR_KINDS = {"sigmoid": 0, "hinge": 1, "square": 2}
 POLICY_REDUCE = {"token": 0, "row": 1, "sum": 2}
-GRAD_CHUNK = 16384          # PCM_GRAD_CHUNK
+GRAD_CHUNK, GRAD_CHUNK_SMALL, GRAD_SMALL = 8192, 1024, 32768      # PCM_GRAD_CHUNK, PCM_GRAD_CHUNK_SMALL and up to how many elements it is for
 
 vp = C.c_void_p
 

@@ -1055,16 +1055,18 @@ class GradSet:
             end_out = max(end_out, b) if is_out else end_out
         self._keep = (grads, dsts)
         src, dst, n, sdt, ddt = np.array(rows, dtype=np.int64).reshape(-1, 5).T
-        per = (n + capi.GRAD_CHUNK - 1) // capi.GRAD_CHUNK
-        self.chunks, self.total = int(per.sum()), int(n.sum())
+        self.total = int(n.sum())
+        cut = capi.GRAD_CHUNK_SMALL if self.total <= capi.GRAD_SMALL else capi.GRAD_CHUNK
+        per = (n + cut - 1) // cut
+        self.chunks = int(per.sum())
         if self.chunks >= 2 ** 31:
             raise ValueError("GradSet: too many elements")
         t = np.repeat(np.arange(len(rows)), per)                                             # tensor of each piece, and its first element
-        start = (np.arange(self.chunks) - np.repeat(np.cumsum(per) - per, per)) * capi.GRAD_CHUNK
+        start = (np.arange(self.chunks) - np.repeat(np.cumsum(per) - per, per)) * cut
         size = np.array([4, 2, 2])                                                           # bytes of an element by PCM_DT_* code
         table = np.zeros(self.chunks, dtype=[("src", "<i8"), ("dst", "<i8"), ("n", "<i4"), ("sdt", "<i4"), ("ddt", "<i4"), ("unused", "<i4")])
         table["src"], table["dst"] = src[t] + start * size[sdt[t]], dst[t] + start * size[ddt[t]]
-        table["n"], table["sdt"], table["ddt"] = np.minimum(n[t] - start, capi.GRAD_CHUNK), sdt[t], ddt[t]
+        table["n"], table["sdt"], table["ddt"] = np.minimum(n[t] - start, cut), sdt[t], ddt[t]
         self._table = torch.from_numpy(table.view(np.uint8)).to(self.device)
         self._stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
 
