@@ -96,7 +96,8 @@ struct PairLoss { double beta, eps; int kind; };
 __device__ __forceinline__ void pair_loss(const PairLoss p, double h, double* loss, double* slope) {
   if (p.kind == PCM_PAIR_SIGMOID) {
     const double s = p.beta * h, e = exp(-fabs(s)), soft = log1p(e);             // -log sig(s) = soft + max(-s, 0)
-    *loss = (1.0 - p.eps) * (soft + fmax(-s, 0.0)) + p.eps * (soft + fmax(s, 0.0));
+    *loss = (1.0 - p.eps) * (soft + fmax(-s, 0.0));
+    if (p.eps > 0.0) *loss += p.eps * (soft + fmax(s, 0.0));                      // (not 0 times infinity)
     *slope = p.beta * ((s >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.eps));
     if (!(s == s)) *loss = s;                                                     // fmax drops a NaN
   } else if (p.kind == PCM_PAIR_HINGE) {
@@ -273,29 +274,35 @@ __device__ __forceinline__ void pair_row_total(const double* part, long row, int
 #pragma unroll
   for (int a = 0; a < R::SUMS; a++) s[a] = pcm_lane_sum(lane < chunks ? part[(row * chunks + lane) * R::SUMS + a] : 0.0);
 }
+// what the threads first, first + step, ... of the pairs add to the loss; their log ratios are written on the way
+template <typename R>
+__device__ __forceinline__ double pair_losses(const R& rows_, const double* part, const PairLoss& pl, float* log_ratio, long pairs, int chunks, long first, long step) {
+  double acc = 0.0;
+  for (long p = first; p < pairs; p += step) {
+    double rho[2], l, s;
+    for (int side = 0; side < 2; side++) {
+      const long row = p + side * pairs;
+      double t[R::SUMS];
+#pragma unroll
+      for (int a = 0; a < R::SUMS; a++) t[a] = 0.0;
+      for (int c = 0; c < chunks; c++)
+#pragma unroll
+        for (int a = 0; a < R::SUMS; a++) t[a] += part[(row * chunks + c) * R::SUMS + a];
+      rho[side] = rows_.rho(row, t);
+      log_ratio[row] = (float)rho[side];
+    }
+    pair_loss(pl, rho[0] - rho[1], &l, &s);
+    acc += l;
+  }
+  return acc;
+}
 template <typename R, int TEAM>
 __global__ __launch_bounds__(256) void pair_grad_kernel(R rows_, const double* part, PairLoss pl, double gscale, float* loss, float* log_ratio, long pairs,
                                                         long n, int chunks, long len) {
   __shared__ double red[4];
   if (blockIdx.x == 0) {
-    double acc = 0.0;
-    for (long p = threadIdx.x; p < pairs; p += 256) {
-      double rho[2], l, s;
-      for (int side = 0; side < 2; side++) {
-        const long row = p + side * pairs;
-        double t[R::SUMS];
-#pragma unroll
-        for (int a = 0; a < R::SUMS; a++) t[a] = 0.0;
-        for (int c = 0; c < chunks; c++)
-#pragma unroll
-          for (int a = 0; a < R::SUMS; a++) t[a] += part[(row * chunks + c) * R::SUMS + a];
-        rho[side] = rows_.rho(row, t);
-        log_ratio[row] = (float)rho[side];
-      }
-      pair_loss(pl, rho[0] - rho[1], &l, &s);
-      acc += l;
-    }
-    acc = pcm_block_sum<256>(acc, red);
+    if (!loss) return;
+    const double acc = pcm_block_sum<256>(pair_losses(rows_, part, pl, log_ratio, pairs, chunks, threadIdx.x, 256), red);
     if (threadIdx.x == 0) loss[0] = (float)(acc / (double)pairs);
     return;
   }
@@ -308,6 +315,20 @@ __global__ __launch_bounds__(256) void pair_grad_kernel(R rows_, const double* p
   pair_loss(pl, rows_.rho(p, up) - rows_.rho(pairs + p, down), &l, &s);
   const double f = (row < pairs ? s * rows_.factor(row, up) : -s * rows_.factor(row, down)) * gscale / (double)pairs;
   rows_.template grad<TEAM>(row, i0, i1, tid, (float)f);
+}
+// more pairs than one workgroup forms the loss of beside the gradient (2048: eight a thread, some 10 us): two launches of their own
+#define PAIR_LOSS_ONE 2048
+#define PAIR_LOSS_PARTS 256
+template <typename R>
+__global__ __launch_bounds__(256) void pair_loss_kernel(R rows_, const double* part, PairLoss pl, float* log_ratio, long pairs, int chunks, double* loss_part) {
+  __shared__ double red[4];
+  const double acc = pcm_block_sum<256>(pair_losses(rows_, part, pl, log_ratio, pairs, chunks, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256), red);
+  if (threadIdx.x == 0) loss_part[blockIdx.x] = acc;
+}
+__global__ __launch_bounds__(256) void pair_loss_finish_kernel(const double* loss_part, int n, long pairs, float* loss) {
+  __shared__ double red[4];
+  const double acc = pcm_block_sum<256>((int)threadIdx.x < n ? loss_part[threadIdx.x] : 0.0, red);
+  if (threadIdx.x == 0) loss[0] = (float)(acc / (double)pairs);
 }
 // few elements: one workgroup takes all pairs in one launch -- a row to a wave, or to all waves where rows are long
 #define PAIR_SMALL_ELEMENTS 32768L
@@ -345,7 +366,7 @@ static bool pair_small(long rows, long n) { return rows <= PAIR_SMALL_ROWS && ro
 static size_t pair_ws_bytes(long rows, long n, int sums) {      // (the 16-bit formats cut into no more chunks than fp32)
   if (pair_small(rows, n)) return 0;
   const RowCut c = row_cut(rows, n, 4);
-  return (size_t)rows * c.chunks * sums * sizeof(double);
+  return ((size_t)rows * c.chunks * sums + (rows > 2 * PAIR_LOSS_ONE ? PAIR_LOSS_PARTS : 0)) * sizeof(double);
 }
 template <typename R>
 static void pair_launch(const R& r, double* part, const PairLoss& pl, double gscale, float* loss, float* log_ratio, long pairs, long n, void* stream) {
@@ -356,12 +377,21 @@ static void pair_launch(const R& r, double* part, const PairLoss& pl, double gsc
   }
   const RowCut c = row_cut(rows, n, R::Dt::VEC);
   const unsigned nb = row_cut_blocks(c, rows), ng = r.wants_grad() ? nb + 1 : 1;
+  const bool apart = pairs > PAIR_LOSS_ONE;
+  float* at_once = apart ? nullptr : loss;
   if (c.team == 64) {
     PCM_LAUNCH((pair_sums_kernel<R, 64>), dim3(nb), dim3(256), 0, stream, r, part, rows, n, c.chunks, c.len);
-    PCM_LAUNCH((pair_grad_kernel<R, 64>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, loss, log_ratio, pairs, n, c.chunks, c.len);
+    PCM_LAUNCH((pair_grad_kernel<R, 64>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, at_once, log_ratio, pairs, n, c.chunks, c.len);
   } else {
     PCM_LAUNCH((pair_sums_kernel<R, 256>), dim3(nb), dim3(256), 0, stream, r, part, rows, n, c.chunks, c.len);
-    PCM_LAUNCH((pair_grad_kernel<R, 256>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, loss, log_ratio, pairs, n, c.chunks, c.len);
+    PCM_LAUNCH((pair_grad_kernel<R, 256>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, at_once, log_ratio, pairs, n, c.chunks, c.len);
+  }
+  if (apart) {
+    double* loss_part = part + rows * c.chunks * R::SUMS;
+    const long want = (pairs + 255) / 256;
+    const int nl = (int)(want < PCM_GRID_CAP(PAIR_LOSS_PARTS) ? want : PCM_GRID_CAP(PAIR_LOSS_PARTS));
+    PCM_LAUNCH(pair_loss_kernel<R>, dim3(nl), dim3(256), 0, stream, r, (const double*)part, pl, log_ratio, pairs, c.chunks, loss_part);
+    PCM_LAUNCH(pair_loss_finish_kernel, dim3(1), dim3(256), 0, stream, (const double*)loss_part, nl, pairs, loss);
   }
 }
 
@@ -796,7 +826,7 @@ extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
   PCM_CHECK(a && a->logp && a->advantages && a->loss && a->stats && a->rows > 0 && a->rows <= AL_MAX_ROWS && a->cols > 0, PCM_EINVAL, "pcm_policy_loss: null/empty or too many rows");
   PCM_CHECK(pcm_dt_ok(a->dtype), PCM_EINVAL, "pcm_policy_loss: unknown element format %d", a->dtype);
   PCM_CHECK(a->reduce == PCM_POLICY_TOKEN || a->reduce == PCM_POLICY_ROW || a->reduce == PCM_POLICY_SUM, PCM_EINVAL, "pcm_policy_loss: unknown reduce %d", a->reduce);
-  PCM_CHECK(a->clip_low >= 0.0 && a->clip_low < 1.0 && a->clip_high >= 0.0 && a->clip_high < 1e30, PCM_EINVAL, "pcm_policy_loss: clip_low must be in [0, 1), clip_high >= 0");
+  PCM_CHECK(a->clip_low >= 0.0 && a->clip_low < 1.0 && a->clip_high >= 0.0, PCM_EINVAL, "pcm_policy_loss: clip_low must be in [0, 1), clip_high >= 0");
   PCM_CHECK(a->kl_coef == 0.0 || a->ref_logp, PCM_EINVAL, "pcm_policy_loss: a KL term needs the reference log-probabilities");
   PCM_CHECK(a->ld_logp >= a->cols && (!a->old_logp || a->ld_old >= a->cols) && (!a->ref_logp || a->ld_ref >= a->cols) && (a->adv_per_row || a->ld_adv >= a->cols) &&
                 (!a->mask || a->ld_mask >= a->cols) && (!a->dlogp || a->ld_dlogp >= a->cols), PCM_EINVAL, "pcm_policy_loss: row stride below the row length");

@@ -964,8 +964,8 @@ def preference_loss(logp, ref_logp, mask=None, lengths=None, beta=0.1, kind="sig
 def policy_loss(logp, advantages, old_logp=None, ref_logp=None, mask=None, lengths=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduce="token",
                 grad_scale=1.0, want_grad=True):
     """Clipped policy loss with a KL term over log-probabilities [N, T] of tokens or sampler steps (rows may be strided):
-    -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(d) - d - 1), r = exp(logp - old_logp), d = ref_logp - logp.  ``old_logp`` None:
-    the policy itself.  advantages fp32 [N] or [N, T]; ``mask`` / ``lengths`` as in preference_loss.  ``reduce``: "token" (mean over all places),
+    -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * (exp(d) - d - 1), r = exp(logp - old_logp), d = ref_logp - logp.  clip_low in [0, 1),
+    clip_high >= 0 or infinite.  ``old_logp`` None: the policy itself.  advantages fp32 [N] or [N, T]; ``mask`` / ``lengths`` as in preference_loss.  ``reduce``: "token" (mean over all places),
     "row" (mean over the N rows of each row's mean) or "sum".
     -> (loss [1], d(grad_scale * loss)/d logp [N, T], stats [4] = objective, KL, share of places held by the clip, places)"""
     name = "policy_loss"
@@ -1068,7 +1068,7 @@ class GradSet:
         table["src"], table["dst"] = src[t] + start * size[sdt[t]], dst[t] + start * size[ddt[t]]
         table["n"], table["sdt"], table["ddt"] = np.minimum(n[t] - start, cut), sdt[t], ddt[t]
         self._table = torch.from_numpy(table.view(np.uint8)).to(self.device)
-        self._stream = torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
+        self._stream = _raw_stream(self.device.index) if self.device.type == "cuda" else None
 
     def _run(self, name, sumsq, *more):
         dev = self.device
@@ -1083,10 +1083,8 @@ class GradSet:
         nb = capi.lib().dll.pcm_grad_norm_workspace_bytes(self.chunks, self.total)
         ws = _scratch(dev, nb)
         _call_on(dev, name, ptr(self._table), self.chunks, self.total, *more, ptr(norm), ptr(sumsq), ptr(ws), nb)
-        if self._stream is not None and not torch.cuda.is_current_stream_capturing():
-            now = torch.cuda.current_stream(dev)
-            if now != self._stream:
-                self._table.record_stream(now)        # the tables were allocated on another stream: not reused before this call is through
+        if self._stream is not None and self._stream != _raw_stream(dev.index) and not torch.cuda.is_current_stream_capturing():
+            self._table.record_stream(torch.cuda.current_stream(dev))      # (allocated on another stream: not reused before this call is through)
         return norm
 
     def norm(self, sumsq=None):

@@ -171,7 +171,7 @@ def case_policy(device, N, T, dtype="f32", masked=False, ragged=False, per_step=
     a = (adv if per_step else adv[:, None].expand(N, T)).double()
     x = (lp.double() - old.double()) if with_old else torch.zeros(N, T, dtype=torch.float64)
     r, d = torch.exp(x), (ref.double() - lp.double()) if with_ref else torch.zeros(N, T, dtype=torch.float64)
-    held = (a > 0) & (x > math.log1p(clip[1])) | (a < 0) & (x < math.log1p(-clip[0]))
+    held = (a > 0) & (x > (math.log1p(clip[1]) if clip[1] < math.inf else math.inf)) | (a < 0) & (x < math.log1p(-clip[0]))
     obj = -torch.minimum(r * a, r.clamp(1 - clip[0], 1 + clip[1]) * a)
     k = torch.special.expm1(d) - d
     slope = torch.where(held, 0.0, -r * a) - kl * torch.special.expm1(d)
@@ -348,6 +348,20 @@ def case_not_a_number(device):
     # an advantage of zero takes a place out of the objective, however far the policy has moved
     far = torch.full((1, 2), 200.0, device=device)
     loss, grad, _ = ops.policy_loss(far, torch.zeros(1, device=device), old_logp=torch.zeros_like(far))
+    assert loss.item() == 0.0 and not grad.cpu().any()
+
+
+def case_infinite_margins(device):
+    """a sample the policy or the reference rules out: the pair's loss is 0 or infinite, its gradient that of the limit, and no 0 times infinity"""
+    inf = float("inf")
+    lp, ref = torch.zeros(4, 3, device=device), torch.zeros(4, 3, device=device)
+    lp[2, 1] = -inf                                   # the rejected sample of pair 0: s = inf
+    lp[1, 0] = -inf                                   # the preferred sample of pair 1: s = -inf
+    loss, grad, ratio = ops.preference_loss(lp, ref, beta=0.5)
+    assert loss.item() == inf and ratio.tolist() == [0.0, -inf, -inf, 0.0]
+    # pair 0: slope 0; pair 1: slope -beta, over two pairs
+    assert grad.cpu().tolist() == [[0.0] * 3, [-0.25] * 3, [0.0] * 3, [0.25] * 3]
+    loss, grad, _ = ops.preference_loss(lp[::2].contiguous(), ref[::2].contiguous(), beta=0.5)
     assert loss.item() == 0.0 and not grad.cpu().any()
 
 

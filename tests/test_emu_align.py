@@ -17,14 +17,15 @@ def _use_emu(request):
 
 @pytest.mark.parametrize("P,n,kw", [(1, 1, {}), (1, 3, dict(kind="square")), (2, 64, dict(eps=0.1, weighted=True)), (3, 255, dict(kind="hinge")),
                                     (2, 1023, dict(dtype="bf16", weighted=True)), (1, 2049, dict(dtype="f16", grad_scale=64.0)),
-                                    (2, 1500, dict(reduce="sum", eps=0.2)), (1, 4100, dict(kind="square", dtype="bf16"))])
+                                    (2, 1500, dict(reduce="sum", eps=0.2)), (1, 4100, dict(kind="square", dtype="bf16")), (2, 9000, dict(weighted=True, eps=0.1)), (1, 20001, dict(dtype="f16")), (40, 500, dict(kind="hinge"))])
 def test_denoise_preference(P, n, kw):
     A.case_denoise_preference("cpu", P, n, **kw)
 
 
 @pytest.mark.parametrize("P,T,kw", [(1, 1, {}), (1, 2, dict(kind="square")), (3, 63, dict(eps=0.1, masked=True)), (2, 65, dict(ragged=True, reduce="mean")),
                                     (3, 257, dict(masked=True, ragged=True, pad=3, dtype="bf16")), (2, 130, dict(dtype="f16", pad=8, masked=True, u8=True)),
-                                    (1, 600, dict(kind="hinge", ragged=True, i64=True)), (4, 5, dict(masked=True, ragged=True, reduce="mean", pad=1))])
+                                    (1, 600, dict(kind="hinge", ragged=True, i64=True)), (4, 5, dict(masked=True, ragged=True, reduce="mean", pad=1)),
+                                    (2500, 2, dict(masked=True)), (3, 11000, dict(masked=True, ragged=True))])
 def test_preference(P, T, kw):
     A.case_preference("cpu", P, T, **kw)
 
@@ -32,7 +33,10 @@ def test_preference(P, T, kw):
 @pytest.mark.parametrize("N,T,kw", [(1, 1, {}), (8, 4, dict(kl=0.04)), (3, 65, dict(masked=True, kl=0.1, reduce="row")), (5, 33, dict(ragged=True, per_step=True)),
                                     (4, 130, dict(masked=True, ragged=True, pad=5, dtype="bf16", kl=0.04)), (3, 77, dict(dtype="f16", reduce="sum", pad=8)),
                                     (2, 40, dict(with_old=False, kl=0.2)), (3, 17, dict(with_ref=True, i64=True, ragged=True, reduce="row")),
-                                    (7, 1, dict(per_step=True, spread=3.0, kl=0.01)), (2, 300, dict(clip=(0.0, 0.0)))])
+                                    (7, 1, dict(per_step=True, spread=3.0, kl=0.01)), (2, 300, dict(clip=(0.0, 0.0))),
+                                    (3, 6000, dict(masked=True, ragged=True, kl=0.1)), (30, 600, dict(masked=True, reduce="row", kl=0.1, pad=1)),
+                                    (4, 5000, dict(masked=True, reduce="row")), (6000, 3, dict(kl=0.1, ragged=True, masked=True)), (5000, 4, dict(reduce="row", masked=True)),
+                                    (2100, 2, dict(per_step=True, pad=2)), (40, 500, dict(clip=(0.9, float("inf")), kl=0.1, spread=1.0))])
 def test_policy(N, T, kw):
     A.case_policy("cpu", N, T, **kw)
 
@@ -47,7 +51,7 @@ def test_policy_where_nothing_counts():
         assert loss.item() == 0.0 and not grad.any() and not stats.any()
 
 
-@pytest.mark.parametrize("B,n,kw", [(1, 1, {}), (3, 63, dict(reduce="sum")), (2, 1025, dict(dtype="bf16")), (2, 700, dict(dtype="f16")), (1, 5000, {})])
+@pytest.mark.parametrize("B,n,kw", [(1, 1, {}), (3, 63, dict(reduce="sum")), (2, 1025, dict(dtype="bf16")), (2, 700, dict(dtype="f16")), (1, 5000, {}), (1, 70001, {}), (40, 1500, dict(dtype="bf16"))])
 def test_transition(B, n, kw):
     A.case_transition("cpu", B, n, **kw)
 
@@ -68,6 +72,10 @@ def test_deterministic():
 
 def test_not_a_number():
     A.case_not_a_number("cpu")
+
+
+def test_infinite_margins():
+    A.case_infinite_margins("cpu")
 
 
 def test_refusals():

@@ -28,7 +28,8 @@ def test_denoise_preference(P, n, kw):
 @pytest.mark.parametrize("P,T,kw", [(1, 1, {}), (1, 2, dict(kind="square")), (3, 63, dict(eps=0.1, masked=True)), (4, 50, {}), (300, 1, {}),
                                     (3, 257, dict(masked=True, ragged=True, pad=3, dtype="bf16")), (2, 4099, dict(dtype="f16", pad=8, masked=True, u8=True)),
                                     (1, 32768, dict(kind="hinge", ragged=True, i64=True)), (9, 1024, dict(masked=True, ragged=True, reduce="mean", pad=1)),
-                                    (1, 70001, dict(masked=True, beta=0.1)), (2, 40000, dict(dtype="bf16", ragged=True)), (700, 40, dict(masked=True))])
+                                    (1, 70001, dict(masked=True, beta=0.1)), (2, 40000, dict(dtype="bf16", ragged=True)), (700, 40, dict(masked=True)),
+                                    (2500, 2, dict(masked=True)), (20000, 1, dict(kind="square")), (3000, 1500, dict(dtype="bf16"))])
 def test_preference(P, T, kw):
     A.case_preference("cuda", P, T, **kw)
 
@@ -37,7 +38,9 @@ def test_preference(P, T, kw):
                                     (64, 1027, dict(masked=True, ragged=True, pad=5, dtype="bf16", kl=0.04)), (33, 777, dict(dtype="f16", reduce="sum", pad=8)),
                                     (2, 40, dict(with_old=False, kl=0.2)), (30, 1700, dict(with_ref=True, i64=True, ragged=True, reduce="row")),
                                     (5000, 1, dict(per_step=True, spread=3.0, kl=0.01)), (2, 300, dict(clip=(0.0, 0.0))), (5000, 7, dict(ragged=True, masked=True, reduce="row")),
-                                    (512, 2048, dict(kl=0.04)), (1, 100003, dict(masked=True, kl=0.04, per_step=True))])
+                                    (40, 500, dict(clip=(0.9, float("inf")), kl=0.1, spread=1.0)), (600, 5000, dict(reduce="row", masked=True, kl=0.1, pad=3)),
+                                    (4, 50001, dict(reduce="row", masked=True, ragged=True)), (9000, 3, dict(reduce="row", masked=True)), (9000, 2, dict(per_step=True, pad=2, dtype="bf16")),
+                                    (6000, 100, dict(ragged=True, i64=True)), (512, 2048, dict(kl=0.04)), (1, 100003, dict(masked=True, kl=0.04, per_step=True))])
 def test_policy(N, T, kw):
     A.case_policy("cuda", N, T, **kw)
 
@@ -66,6 +69,10 @@ def test_deterministic():
 
 def test_not_a_number():
     A.case_not_a_number("cuda")
+
+
+def test_infinite_margins():
+    A.case_infinite_margins("cuda")
 
 
 def test_refusals():
