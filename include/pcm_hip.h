@@ -543,9 +543,9 @@ typedef struct {
   double clip_low, clip_high, kl_coef, grad_scale;
   int dtype, reduce, adv_per_row, lengths_i64;
 } pcm_policy_args;
-size_t pcm_policy_loss_workspace_bytes(long rows, long cols);
+size_t pcm_policy_loss_workspace_bytes(long rows, long cols, int reduce);
 int pcm_policy_loss(const pcm_policy_args* a, void* stream);
-/* Global norm of gradients held in many tensors, and their clipping (torch.nn.utils' rule, as in pcm_adamw_clip_step):
+/* Global norm of gradients held in many tensors, and their clipping (by the rule of pcm_adamw_clip_step):
  *   sumsq = sum g^2 (fp64), norm = sqrt(sumsq);   dst = src * min(1, max_norm / (norm + 1e-6))
  * `chunks` is a table in DEVICE memory: the tensors cut into pieces of n <= PCM_GRAD_CHUNK consecutive elements, `total` elements in all.
  * dst may be src (then nothing is written when nothing has to be clipped) or a place apart; its format may be another one.  Pieces that are

@@ -1,6 +1,8 @@
 // pcm-build-flags: -Xclang -target-feature -Xclang -packed-fp32-ops
 // Alignment of a distilled student: preference losses over paired log ratios, the clipped policy loss with its KL term, and the log-probability
-// of a noisy sampler transition, each with its gradient.  Everything here is bound by memory: a few operations per element read.
+// of a noisy sampler transition, each with its gradient.  Large calls are bound by memory (a few operations per element read; 60 in the policy loss,
+// which is why its exponentials are counted), small ones by their launches: about 4 us of host time each.  Times below are of one MI355X, whose
+// large copies run at 5.1 TB/s and whose reads alone reach 6.8.
 //
 // Elements are formed in fp32; every sum over elements, rows or tokens is carried in fp64 and in an order fixed by the launch (partial sums in the
 // caller's workspace, added up by index), so results are bitwise the same run to run.
@@ -33,15 +35,17 @@ __device__ __forceinline__ bool row_cut_place(long block, long rows, int chunks,
   return true;
 }
 
-// ---- log-probability of x ~ N(mean, std^2) per row:  -1/2 sum ((x - mean) / std)^2 - n log std - n/2 log 2 pi   (/ n) ----
+// ---- Log-probability of a transition.  Forward: one pass, 8 bytes read an element (fp32); 64 rows of 262144 in two launches, 26 us.  Gradient: elementwise
+// in the forward's cut of rows, so that std and dlogp are read once a workgroup; 64 rows of 262144 fp32 in 31 us, 201 MB at 6.4 TB/s.
+// x ~ N(mean, std^2) per row:  -1/2 sum ((x - mean) / std)^2 - n log std - n/2 log 2 pi   (/ n) ----
 #define LOG_2PI 1.8378770664093454836
 __device__ __forceinline__ float transition_value(double acc, double s, long n, int mean_reduce) {
   const double per = -0.5 * acc / (s * s * (double)n) - log(s) - 0.5 * LOG_2PI;
   return (float)(mean_reduce ? per : per * (double)n);
 }
 template <typename Dt, int TEAM>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void transition_fwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std, float* logp, double* part,
-                                                             long rows, long n, int chunks, long len, int mean_reduce) {
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void transition_fwd_kernel(const typename Dt::raw* x, const typename Dt::raw* mean, const float* std,
+                                                                                      float* logp, double* part, long rows, long n, int chunks, long len, int mean_reduce) {
   __shared__ double red[16];
   long row; int chunk, tid;
   if (!row_cut_place<TEAM>(blockIdx.x, rows, chunks, &row, &chunk, &tid)) return;
@@ -254,7 +258,10 @@ struct TokenRows {
   bool wants_grad() const { return dlogp != nullptr; }
 };
 // Two launches: (1) partial sums of every (row, chunk); (2) the gradient, where each team adds up the partial sums of its pair again instead of
-// waiting for a launch that does it once -- at most 2 x 64 numbers out of L2 -- and the first workgroup forms the mean loss.
+// waiting for a launch that does it once -- at most 2 x 64 numbers out of L2 -- and the first workgroup forms the mean loss.  The gradient has to wait for
+// both rows of its pair, so t and p are read twice: 64 pairs of 262144 fp32, (1) 402 MB in 60 us (6.7 TB/s), (2) 268 MB in and 134 out in 64 us
+// (6.3 TB/s).  Launching groups of pairs whose rows stay in the 256 MB cache for (2) was slower, 143 us and more: every launch ends with workgroups
+// that wait for the last loads.
 template <typename R, int TEAM>
 __global__ __launch_bounds__(256) void pair_sums_kernel(R rows_, double* part, long rows, long n, int chunks, long len) {
   __shared__ double red[4];
@@ -330,21 +337,36 @@ __global__ __launch_bounds__(256) void pair_loss_finish_kernel(const double* los
   const double acc = pcm_block_sum<256>((int)threadIdx.x < n ? loss_part[threadIdx.x] : 0.0, red);
   if (threadIdx.x == 0) loss[0] = (float)(acc / (double)pairs);
 }
-// few elements: one workgroup takes all pairs in one launch -- a row to a wave, or to all waves where rows are long
+// few elements: one workgroup takes all pairs in one launch -- a row to a wave, or to half of the waves where rows are long.  At the limit (one pair of
+// 16384 fp32) 14.2 us among others against 18.8 in two launches, alone 30.7 against 31.3; at twice as much alone 38 against 33
 #define PAIR_SMALL_ELEMENTS 32768L
 #define PAIR_SMALL_ROWS 128
 template <typename R>
 __global__ __launch_bounds__(1024) void pair_small_kernel(R rows_, PairLoss pl, double gscale, float* loss, float* log_ratio, int pairs, int n, int want_grad) {
-  __shared__ double red[16], rho[PAIR_SMALL_ROWS], factor[PAIR_SMALL_ROWS], slope[PAIR_SMALL_ROWS / 2];
+  __shared__ double red[16 * R::SUMS], rho[PAIR_SMALL_ROWS], factor[PAIR_SMALL_ROWS], slope[PAIR_SMALL_ROWS / 2];
   const int rows = 2 * pairs, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const bool by_wave = n <= 1024;
+  const int team = by_wave ? wave : wave >> 3, teams = by_wave ? 16 : 2, half = threadIdx.x & 511;
   double s[R::SUMS];
-  for (int row = by_wave ? wave : 0; row < rows; row += by_wave ? 16 : 1) {
+  for (int row = team; row < rows; row += teams) {      // (rows is even: both halves of the workgroup take as many)
     if (by_wave) rows_.template sums<64>(row, 0, n, lane, s);
-    else rows_.template sums<1024>(row, 0, n, threadIdx.x, s);
+    else rows_.template sums<512>(row, 0, n, half, s);
 #pragma unroll
-    for (int a = 0; a < R::SUMS; a++) s[a] = by_wave ? pcm_lane_sum(s[a]) : pcm_block_sum<1024>(s[a], red);
-    if (by_wave ? lane == 0 : threadIdx.x == 0) {
+    for (int a = 0; a < R::SUMS; a++) s[a] = pcm_lane_sum(s[a]);
+    if (!by_wave) {
+      __syncthreads();
+      if (lane == 0)
+#pragma unroll
+        for (int a = 0; a < R::SUMS; a++) red[wave * R::SUMS + a] = s[a];
+      __syncthreads();
+#pragma unroll
+      for (int a = 0; a < R::SUMS; a++) {
+        s[a] = red[team * 8 * R::SUMS + a];
+#pragma unroll
+        for (int w = 1; w < 8; w++) s[a] += red[(team * 8 + w) * R::SUMS + a];
+      }
+    }
+    if (by_wave ? lane == 0 : half == 0) {
       rho[row] = rows_.rho(row, s); factor[row] = rows_.factor(row, s);
       log_ratio[row] = (float)rho[row];
     }
@@ -355,10 +377,10 @@ __global__ __launch_bounds__(1024) void pair_small_kernel(R rows_, PairLoss pl, 
   l = pcm_block_sum<1024>(l, red);
   if (threadIdx.x == 0) loss[0] = (float)(l / (double)pairs);
   if (!want_grad) return;
-  for (int row = by_wave ? wave : 0; row < rows; row += by_wave ? 16 : 1) {
+  for (int row = team; row < rows; row += teams) {
     const float f = (float)((row < pairs ? slope[row] : -slope[row - pairs]) * factor[row] * gscale / (double)pairs);
     if (by_wave) rows_.template grad<64>(row, 0, n, lane, f);
-    else rows_.template grad<1024>(row, 0, n, threadIdx.x, f);
+    else rows_.template grad<512>(row, 0, n, half, f);
   }
 }
 static bool pair_small(long rows, long n) { return rows <= PAIR_SMALL_ROWS && rows * n <= PAIR_SMALL_ELEMENTS; }
@@ -639,7 +661,8 @@ __device__ __forceinline__ void policy_store(const double (&s)[POLICY_SUMS], dou
 #pragma unroll
     for (int k = 0; k < POLICY_SUMS; k++) part[(long)blockIdx.x * POLICY_SUMS + k] = s[k];
 }
-// (256, 8): 8 waves to a SIMD, so that all 2048 workgroups are resident at once; a workgroup takes consecutive groups (a strided grid reads 15 % slower)
+// (256, 8): 8 waves to a SIMD, so that all 2048 workgroups are resident at once; a workgroup takes consecutive groups (a strided grid reads 15 % slower).
+// 2048 x 8192 fp32 with old and reference log-probabilities: 268 MB in 50 us; with ragged rows, 194 MB, 42 us (without its arithmetic 13 % less).
 template <bool KL, bool NARROW, typename Dt>
 __global__ __launch_bounds__(256, 8) void policy_main_kernel(PolicyRows<Dt> a, PolicyWeight pw, double* part) {
   __shared__ double red[4 * POLICY_SUMS];
@@ -678,7 +701,8 @@ __global__ __launch_bounds__(256) void policy_finish_kernel(const double* part, 
   pcm_block_sums<256>(s, red);
   if (threadIdx.x == 0) policy_result(s, kl, loss, stats);
 }
-// few places: one workgroup counts, forms loss and gradient, and adds up, in one launch
+// few places: one workgroup counts, forms loss and gradient, and adds up, in one launch.  At the limit (64 x 256 bf16, masked) 17.7 us among others against
+// 24.6 in three launches, alone 39 against 36; at twice as much 23.2 against 24.5 and 47 against 36
 #define POLICY_SMALL_PLACES 16384
 #define POLICY_SMALL_ROWS 2048
 template <bool KL, bool NARROW, typename Dt>
@@ -711,8 +735,8 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(PolicyRows<Dt> a, in
 // ---- entry points ----
 #define AL_MAX_LD 4294967296L
 #define AL_MAX_ROWS 16777216L       /* 64 chunks of a row at the most: a grid stays below 2^31 workgroups */
-// the forward pass takes a row to a workgroup of 1024 where rows are too few for one chunk each but short enough: one launch instead of two, 16 rows of
-// 16384 in 2.3 us against 3.1 + 2.5
+// the forward pass takes a row to a workgroup of 1024 where rows are too few for one chunk each but short enough: one launch instead of two.  16 rows of
+// 16384: 4.2 us against 3.1 + 2.5 and 4 us less host time; one row of 65536 among others 12 us against 16, of 131072 alone 28 against 26
 static RowCut transition_cut(long rows, long n, int vec) {
   RowCut c = row_cut(rows, n, vec);
   if (c.chunks > 1 && n <= ROW_TEAM_MAX) { c.team = 1024; c.chunks = 1; c.len = n; }
@@ -752,8 +776,9 @@ extern "C" int pcm_transition_logprob_bwd(const void* x, const void* mean, const
     typedef const typename Dt::raw* cp;
     const RowCut c = row_cut(rows, n, Dt::VEC);
     const dim3 grid(row_cut_blocks(c, rows));
-    if (c.team == 64) PCM_LAUNCH((transition_bwd_kernel<Dt, 64>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, c.chunks, c.len, mean_reduce);
-    else PCM_LAUNCH((transition_bwd_kernel<Dt, 256>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, (typename Dt::raw*)dmean, rows, n, c.chunks, c.len, mean_reduce);
+    typename Dt::raw* d = (typename Dt::raw*)dmean;
+    if (c.team == 64) PCM_LAUNCH((transition_bwd_kernel<Dt, 64>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, d, rows, n, c.chunks, c.len, mean_reduce);
+    else PCM_LAUNCH((transition_bwd_kernel<Dt, 256>), grid, dim3(256), 0, stream, (cp)x, (cp)mean, std, dlogp, d, rows, n, c.chunks, c.len, mean_reduce);
   });
   return pcm_post_launch("pcm_transition_logprob_bwd");
 }
@@ -810,9 +835,11 @@ static bool policy_small(long rows, long cols) { return rows <= POLICY_SMALL_ROW
 // a workgroup to a row: rows long enough to keep it busy, and enough of them for the chip or none too long for one
 static bool policy_by_row(int reduce, long rows, long cols) { return reduce == PCM_POLICY_ROW && cols >= 512 && (rows >= 512 || cols <= 4096); }
 #define POLICY_COUNT_PARTS 512
-extern "C" size_t pcm_policy_loss_workspace_bytes(long rows, long cols) {      // partial counts or weights of rows, then the partial sums
+// partial counts, or weights of rows
+static long policy_counts(long rows, int reduce) { return reduce == PCM_POLICY_ROW && rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS; }
+extern "C" size_t pcm_policy_loss_workspace_bytes(long rows, long cols, int reduce) {
   if (rows <= 0 || cols <= 0 || policy_small(rows, cols)) return 0;
-  return ((rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS) + POLICY_SUMS * 2048) * sizeof(double);
+  return (size_t)(policy_counts(rows, reduce) + POLICY_SUMS * 2048) * sizeof(double);
 }
 #define POLICY_LAUNCH(kernel, grid, block, ...)                                                                              \
   do {                                                                                                                       \
@@ -832,7 +859,7 @@ extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
                 (!a->mask || a->ld_mask >= a->cols) && (!a->dlogp || a->ld_dlogp >= a->cols), PCM_EINVAL, "pcm_policy_loss: row stride below the row length");
   PCM_CHECK(a->cols < 2147483648L - 65536 && a->ld_logp < AL_MAX_LD && a->ld_old < AL_MAX_LD && a->ld_ref < AL_MAX_LD && a->ld_adv < AL_MAX_LD && a->ld_mask < AL_MAX_LD &&
                 a->ld_dlogp < AL_MAX_LD, PCM_EINVAL, "pcm_policy_loss: row stride of 2^32 elements or more");
-  const size_t need = pcm_policy_loss_workspace_bytes(a->rows, a->cols);
+  const size_t need = pcm_policy_loss_workspace_bytes(a->rows, a->cols, a->reduce);
   PCM_CHECK(need == 0 || (a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= need), PCM_EINVAL,
             "pcm_policy_loss: workspace too small or not 8-byte aligned");
   const Places pc = {a->mask, a->ld_mask, a->lengths, a->lengths_i64, a->cols};
@@ -850,7 +877,7 @@ extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
       POLICY_LAUNCH(policy_small_kernel, dim3(1), dim3(1024), r, reduce, a->kl_coef, a->loss, a->stats);
       return;
     }
-    double *counts = (double*)a->workspace, *part = counts + (rows > POLICY_COUNT_PARTS ? rows : POLICY_COUNT_PARTS);
+    double *counts = (double*)a->workspace, *part = counts + policy_counts(rows, a->reduce);
     int nb = al_blocks(rows * gpr);
     if (by_row) {
       nb = (int)(rows < PCM_GRID_CAP(2048) ? rows : PCM_GRID_CAP(2048));

@@ -229,7 +229,7 @@ class Lib:
         for name, argt in (("pcm_rowdot_bwd_workspace_bytes", [C.c_long, C.c_int]), ("pcm_groupnorm_param_grad_workspace_bytes", [C.c_int] * 4),
                            ("pcm_mod_grad_workspace_bytes", [C.c_int] * 3),        # abi 5
                            ("pcm_transition_logprob_workspace_bytes", [C.c_long] * 2), ("pcm_denoise_preference_loss_workspace_bytes", [C.c_long] * 2),
-                           ("pcm_preference_loss_workspace_bytes", [C.c_long] * 2), ("pcm_policy_loss_workspace_bytes", [C.c_long] * 2),
+                           ("pcm_preference_loss_workspace_bytes", [C.c_long] * 2), ("pcm_policy_loss_workspace_bytes", [C.c_long, C.c_long, C.c_int]),
                            ("pcm_grad_norm_workspace_bytes", [C.c_int, C.c_long])):        # abi 6
             f = getattr(self.dll, name, None)
             if f is not None:

@@ -853,6 +853,10 @@ def _choice(name, what, value, table):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _call_on(dev, name, *args):
     """the call on ``dev``'s current stream, whichever device is the current one"""
     if dev.type != "cuda":
@@ -891,7 +895,7 @@ def transition_logprob(x, mean, std, reduce="mean"):
     out = torch.empty(rows, dtype=torch.float32, device=dev)
     nb = capi.lib().dll.pcm_transition_logprob_workspace_bytes(rows, n)
     ws = _scratch(dev, nb)
-    _call_on(dev, "pcm_transition_logprob", ptr(x), ptr(mean), ptr(std), dt, m, ptr(out), rows, n, ptr(ws), nb)
+    _call_on(dev, "pcm_transition_logprob", _addr(x), _addr(mean), _addr(std), dt, m, _addr(out), rows, n, _addr(ws), nb)
     return out
 
 
@@ -900,7 +904,7 @@ def transition_logprob_bwd(x, mean, std, dlogp, reduce="mean"):
     m = _choice("transition_logprob_bwd", "reduce", reduce, {"mean": 1, "sum": 0})
     dev, dt, rows, n = _transition_args("transition_logprob_bwd", x, mean, std, dlogp=dlogp)
     dmean = torch.empty_like(mean)
-    _call_on(dev, "pcm_transition_logprob_bwd", ptr(x), ptr(mean), ptr(std), ptr(dlogp), dt, m, ptr(dmean), rows, n)
+    _call_on(dev, "pcm_transition_logprob_bwd", _addr(x), _addr(mean), _addr(std), _addr(dlogp), dt, m, _addr(dmean), rows, n)
     return dmean
 
 
@@ -930,8 +934,8 @@ def denoise_preference_loss(pred, ref_pred, target, weight=None, beta=2000.0, ki
     dpred = torch.empty_like(pred) if want_grad else None
     nb = capi.lib().dll.pcm_denoise_preference_loss_workspace_bytes(rows // 2, n)
     ws = _scratch(dev, nb)
-    a = capi.DenoisePreferenceArgs(ptr(pred), ptr(ref_pred), ptr(target), ptr(weight), ptr(dpred), ptr(loss), ptr(ratio), ptr(ws), nb, rows // 2, n,
-                                   beta, label_smoothing, grad_scale, dt, kd, m)
+    a = capi.DenoisePreferenceArgs(_addr(pred), _addr(ref_pred), _addr(target), _addr(weight), _addr(dpred), _addr(loss), _addr(ratio), _addr(ws), nb,
+                                   rows // 2, n, beta, label_smoothing, grad_scale, dt, kd, m)
     _call_on(dev, "pcm_denoise_preference_loss", C.byref(a))
     return loss, dpred, ratio
 
@@ -955,7 +959,8 @@ def preference_loss(logp, ref_logp, mask=None, lengths=None, beta=0.1, kind="sig
     dlogp = torch.empty(rows, cols, dtype=logp.dtype, device=dev) if want_grad else None
     nb = capi.lib().dll.pcm_preference_loss_workspace_bytes(rows // 2, cols)
     ws = _scratch(dev, nb)
-    a = capi.PreferenceArgs(ptr(logp), ptr(ref_logp), ptr(mask), ptr(lengths), ptr(dlogp), ptr(loss), ptr(ratio), ptr(ws), nb, rows // 2, cols,
+    a = capi.PreferenceArgs(_addr(logp), _addr(ref_logp), _addr(mask), _addr(lengths), _addr(dlogp), _addr(loss), _addr(ratio), _addr(ws), nb,
+                            rows // 2, cols,
                             ldl, ldr, ldm, cols, beta, label_smoothing, grad_scale, dt, kd, m, l64)
     _call_on(dev, "pcm_preference_loss", C.byref(a))
     return loss, dlogp, ratio
@@ -990,10 +995,10 @@ def policy_loss(logp, advantages, old_logp=None, ref_logp=None, mask=None, lengt
     loss = torch.empty(1, dtype=torch.float32, device=dev)
     stats = torch.empty(4, dtype=torch.float32, device=dev)
     dlogp = torch.empty(rows, cols, dtype=logp.dtype, device=dev) if want_grad else None
-    nb = capi.lib().dll.pcm_policy_loss_workspace_bytes(rows, cols)
+    nb = capi.lib().dll.pcm_policy_loss_workspace_bytes(rows, cols, rd)
     ws = _scratch(dev, nb)
-    a = capi.PolicyArgs(ptr(logp), ptr(old_logp), ptr(ref_logp), ptr(advantages), ptr(mask), ptr(lengths), ptr(dlogp), ptr(loss), ptr(stats), ptr(ws), nb,
-                        rows, cols, ldl, ldo, ldr, lda, ldm, cols, clip_low, clip_high, kl_coef, grad_scale, dt, rd, int(per_row), l64)
+    a = capi.PolicyArgs(_addr(logp), _addr(old_logp), _addr(ref_logp), _addr(advantages), _addr(mask), _addr(lengths), _addr(dlogp), _addr(loss),
+                        _addr(stats), _addr(ws), nb, rows, cols, ldl, ldo, ldr, lda, ldm, cols, clip_low, clip_high, kl_coef, grad_scale, dt, rd, int(per_row), l64)
     _call_on(dev, "pcm_policy_loss", C.byref(a))
     return loss, dlogp, stats
 
@@ -1025,36 +1030,35 @@ class GradSet:
             raise ValueError(f"GradSet: {len(grads)} gradients but {len(dsts)} outputs")
         if not grads:
             raise ValueError("GradSet: no gradients")
-        if not all(isinstance(t, torch.Tensor) for t in grads + dsts):
+        every = grads if out is None else grads + dsts
+        if not all(isinstance(t, torch.Tensor) for t in every):
             raise TypeError("GradSet: gradients and outputs must be tensors")
-        self.device = _one_place("GradSet", **{f"tensor {i}": t for i, t in enumerate(grads + (dsts if out is not None else []))})
-        spans, rows = [], []
+        self.device = _one_place("GradSet", gradient=grads[0])
+        rows = []
         for i, (g, o) in enumerate(zip(grads, dsts)):
-            for t in (g, o):
-                if t.dtype not in capi.DT_CODES:
-                    raise TypeError(f"GradSet: tensor {i} must be float32, bfloat16 or float16, got {t.dtype}")
+            if g.device != self.device or o.device != self.device:
+                raise ValueError(f"GradSet: tensor {i} or its output is not on {self.device}")
+            if g.dtype not in capi.DT_CODES or o.dtype not in capi.DT_CODES:
+                raise TypeError(f"GradSet: tensor {i} must be float32, bfloat16 or float16, got {g.dtype} and {o.dtype}")
             if g.shape != o.shape:
                 raise ValueError(f"GradSet: output {i} must be {list(g.shape)}, got {list(o.shape)}")
-            if g.numel() == 0:
-                continue
-            order = _dense_order(g)
-            if order is None or _dense_order(o) != order:
-                raise ValueError(f"GradSet: gradient {i} and its output must each fill their memory without gaps, in the same element order")
-            s0, d0 = g.data_ptr(), o.data_ptr()
-            s1, d1 = s0 + g.numel() * g.element_size(), d0 + o.numel() * o.element_size()
-            own = s0 == d0 and g.dtype == o.dtype
-            spans.append((d0, d1, True))
-            if not own:
-                spans.append((s0, s1, False))
-            rows.append((s0, d0, g.numel(), capi.DT_CODES[g.dtype], capi.DT_CODES[o.dtype]))
-        end_any = end_out = 0
-        for a, b, is_out in sorted(spans):
-            if a < (end_any if is_out else end_out):
-                raise ValueError("GradSet: an output overlaps another output or a gradient that is not its own")
-            end_any = max(end_any, b)
-            end_out = max(end_out, b) if is_out else end_out
+            if not (g.is_contiguous() and o.is_contiguous()):
+                order = _dense_order(g)
+                if order is None or _dense_order(o) != order:
+                    raise ValueError(f"GradSet: gradient {i} and its output must each fill their memory without gaps, in the same element order")
+            if g.numel():
+                rows.append((g.data_ptr(), o.data_ptr(), g.numel(), capi.DT_CODES[g.dtype], capi.DT_CODES[o.dtype]))
         self._keep = (grads, dsts)
         src, dst, n, sdt, ddt = np.array(rows, dtype=np.int64).reshape(-1, 5).T
+        size = np.array([4, 2, 2])                                                           # bytes of an element by PCM_DT_* code
+        # outputs apart from one another, and from the gradients that are not clipped in place
+        order = np.argsort(dst)
+        d0, d1 = dst[order], (dst + n * size[ddt])[order]
+        apart = (src != dst) | (sdt != ddt)
+        s0, s1 = src[apart], (src + n * size[sdt])[apart]
+        below = np.searchsorted(d0, s1) - 1                                                  # the last output that begins below a gradient's end
+        if (d0[1:] < d1[:-1]).any() or ((below >= 0) & (d1[below] > s0)).any():
+            raise ValueError("GradSet: an output overlaps another output or a gradient that is not its own")
         self.total = int(n.sum())
         cut = capi.GRAD_CHUNK_SMALL if self.total <= capi.GRAD_SMALL else capi.GRAD_CHUNK
         per = (n + cut - 1) // cut
@@ -1063,7 +1067,6 @@ class GradSet:
             raise ValueError("GradSet: too many elements")
         t = np.repeat(np.arange(len(rows)), per)                                             # tensor of each piece, and its first element
         start = (np.arange(self.chunks) - np.repeat(np.cumsum(per) - per, per)) * cut
-        size = np.array([4, 2, 2])                                                           # bytes of an element by PCM_DT_* code
         table = np.zeros(self.chunks, dtype=[("src", "<i8"), ("dst", "<i8"), ("n", "<i4"), ("sdt", "<i4"), ("ddt", "<i4"), ("unused", "<i4")])
         table["src"], table["dst"] = src[t] + start * size[sdt[t]], dst[t] + start * size[ddt[t]]
         table["n"], table["sdt"], table["ddt"] = np.minimum(n[t] - start, cut), sdt[t], ddt[t]
@@ -1082,7 +1085,7 @@ class GradSet:
         norm = torch.empty(1, dtype=torch.float32, device=dev)
         nb = capi.lib().dll.pcm_grad_norm_workspace_bytes(self.chunks, self.total)
         ws = _scratch(dev, nb)
-        _call_on(dev, name, ptr(self._table), self.chunks, self.total, *more, ptr(norm), ptr(sumsq), ptr(ws), nb)
+        _call_on(dev, name, _addr(self._table), self.chunks, self.total, *more, _addr(norm), _addr(sumsq), _addr(ws), nb)
         if self._stream is not None and self._stream != _raw_stream(dev.index) and not torch.cuda.is_current_stream_capturing():
             self._table.record_stream(torch.cuda.current_stream(dev))      # (allocated on another stream: not reused before this call is through)
         return norm

@@ -306,6 +306,67 @@ def case_policy_run(device, B=3, steps=4, n=24, seed=0):
     close(torch.cat(grads), th.grad * f, 2 * (dlogp_tol * reach + 64 * U * reach), "gradient of theta")
 
 
+def case_preference_step(device, hw=8, seed=0):
+    """the operators as they are used together: one preference step of the student against its own frozen base -- forward of preferred and rejected
+    samples, loss and gradient, LoRA backward, global norm over the factors' gradients, AdamW on it, clipping of a copy -- against the oracle's autograd"""
+    from oracle import unet_sd15 as O
+    from pcm_amd.model import LoraState, UNet, UNetWeights
+    from pcm_amd.unet_spec import UNetConfig
+    kw = dict(block_out_channels=(64, 128, 128), cross_attention_dim=64, heads=2, norm_num_groups=32)
+    oc, pc = O.UNetConfig(**kw), UNetConfig(**kw)
+    sd = O.init_state_dict(oc, 0)
+    g = torch.Generator().manual_seed(seed)
+    latents, noise = torch.randn(2, 4, hw, hw, generator=g), torch.randn(2, 4, hw, hw, generator=g)
+    ctx, t, beta = torch.randn(2, 7, 64, generator=g), torch.tensor([419, 419]), 1.0
+    W, lora = UNetWeights(pc, sd, device), LoraState(pc, 64, 8.0, device, seed=1, b_std=0.05)
+    olora = {k: (lora.A_peft(m).detach().cpu().clone().requires_grad_(), m.B.detach().cpu().clone().requires_grad_()) for k, m in lora.modules.items()}
+    x, dev = (0.6 * latents + 0.8 * noise), lambda v: v.to(device)      # noqa: E731
+    student, base = UNet(W, lora), UNet(W, None)
+    eps, tape = student.forward(dev(x), dev(t), dev(ctx), save=True)
+    ref = base.forward(dev(x), dev(t), dev(ctx))
+    loss, d_eps, ratio = ops.denoise_preference_loss(eps, ref, dev(noise), beta=beta)
+    lora.zero_grad()
+    student.backward(d_eps, tape)
+
+    oeps, oref = O.unet_forward(oc, sd, x, t, ctx, olora, 8.0), O.unet_forward(oc, sd, x, t, ctx).detach()
+    n = oeps[0].numel()
+    rho = -(((noise - oeps).double() ** 2 - (noise - oref).double() ** 2).flatten(1).sum(1)) / n
+    oloss = -torch.nn.functional.logsigmoid(beta * (rho[0] - rho[1]))
+    oloss.backward()
+    rho, oloss = rho.detach(), oloss.detach()
+    # the operator on the predictions it was given, exactly; against the oracle's predictions, by how far the log ratios are apart
+    e, r, no = eps.double().cpu(), ref.double().cpu(), noise.double()
+    own = -(((no - e) ** 2 - (no - r) ** 2).flatten(1).sum(1)) / n
+    close(ratio, own, 12 * U * ((no - e) ** 2 + (no - r) ** 2).flatten(1).sum(1) / n + U * own.abs(), "log ratios")
+    gap = float(((own[0] - own[1]) - (rho[0] - rho[1])).abs())
+    assert abs(loss.item() - oloss.item()) <= beta * gap + 1e-6, (loss.item(), oloss.item(), gap)
+    # the slope is off by at most beta gap / 4 of beta; the network's bf16 backward by 5 % (the bound of its own test on this width)
+    slope = float(torch.sigmoid(-beta * (rho[0] - rho[1])))
+    num = sum(float(((got.cpu() - want.grad.view_as(got)) ** 2).sum()) for k, m in lora.modules.items()
+              for got, want in ((lora.gA_peft(m), olora[k][0]), (m.gB, olora[k][1])))
+    den = sum(float((want.grad ** 2).sum()) for pair in olora.values() for want in pair)
+    print("preference step: LoRA gradient rel err %.3e, margin off by %.3e" % ((num / den) ** 0.5, gap))
+    assert (num / den) ** 0.5 < 0.05 + beta * gap / 4 / slope
+    # norm over the factors' gradients (views of the flat buffer), and the optimizer step that takes its square
+    factors = [t for m in lora.modules.values() for t in (m.gA, m.gB)]
+    copies = [torch.empty_like(t) for t in factors]
+    gs = ops.GradSet(factors, out=copies)
+    flat = (lora.grads.double() ** 2).sum().item()
+    norm = gs.norm(sumsq=lora.gradsq)
+    close(lora.gradsq, torch.tensor([flat], dtype=torch.float64), 1e-12 * flat, "sum of squares")
+    norm2, c = gs.clip(0.5 * flat ** 0.5), 0.5 * flat ** 0.5 / (flat ** 0.5 + 1e-6)
+    assert torch.equal(norm, norm2)
+    for a, b in zip(copies, factors):
+        want = b.double().cpu() * c
+        close(a, want, out_tol(want, 2 * U * want.abs(), torch.float32), "clipped factor gradient")
+    before, max_norm, lr, wd = lora.params.clone(), 0.5 * flat ** 0.5, 1e-4, 1e-2
+    ops.adamw_clip_step(lora.params, lora.grads, lora.exp_avg, lora.exp_avg_sq, lora.gradsq, max_norm, lr, 0.9, 0.999, 1e-8, wd, 1)
+    clipped = lora.grads.double().cpu() * c
+    want = before.double().cpu() * (1 - lr * wd) - lr * clipped / (clipped.abs() + 1e-8)      # the first step: m / bc1 = g, sqrt(v / bc2) = |g|
+    # g / (|g| + eps) to a few fp32 roundings where |g| is not lost against eps
+    close(lora.params, want, 16 * U * (before.double().cpu().abs() + lr) + lr * 64 * U, "parameters after the step")
+
+
 def case_deterministic(device, big=False):
     """the same call twice gives the same bits"""
     g = torch.Generator().manual_seed(5)

@@ -66,6 +66,14 @@ def test_policy_run():
     A.case_policy_run("cpu")
 
 
+@pytest.mark.slow
+def test_preference_step():
+    from pcm_amd import precision
+    if capi.lib().act_dtype == 0:            # (the network's buffers are in the process's one 16-bit format, bfloat16)
+        assert precision.precision() == "bf16"
+        A.case_preference_step("cpu")
+
+
 def test_deterministic():
     A.case_deterministic("cpu")
 

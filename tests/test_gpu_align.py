@@ -63,6 +63,10 @@ def test_policy_run():
     A.case_policy_run("cuda", B=5, steps=8, n=256, seed=1)
 
 
+def test_preference_step():
+    A.case_preference_step("cuda", hw=16)
+
+
 def test_deterministic():
     A.case_deterministic("cuda", big=True)
 
