@@ -486,7 +486,7 @@ struct PolicyRows {
   raw* dlogp;                       // NULL: no gradient
   long ld_d;
   int rows, gpr;                    // groups of a row
-  float gscale;
+  double gscale;
 };
 // what a launch adds up: objective, KL (both weighted), places held by the clip, places
 enum { POLICY_OBJ, POLICY_KL, POLICY_HELD, POLICY_COUNT, POLICY_SUMS };
@@ -501,7 +501,7 @@ struct PolicyRow { int len; double w; float wg; PolicySide side; };
 template <typename Dt>
 __device__ __forceinline__ PolicyRow policy_row(const PolicyRows<Dt>& a, int row, int len, double w) {
   PolicyRow r;
-  r.len = len; r.w = w; r.wg = (float)(w * (double)a.gscale);
+  r.len = len; r.w = w; r.wg = (float)(w * a.gscale);
   if (!a.ld_adv) r.side = PolicySide(a.con, a.adv[row]);
   return r;
 }
@@ -872,7 +872,7 @@ extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
     const PolicyRows<Dt> r = {(cp)a->logp, (cp)(a->old_logp ? a->old_logp : a->logp), (cp)a->ref_logp, a->ld_logp, a->old_logp ? a->ld_old : a->ld_logp, a->ld_ref,
-                              a->advantages, a->adv_per_row ? 0 : a->ld_adv, pc, con, (typename Dt::raw*)a->dlogp, a->ld_dlogp, (int)rows, gpr, (float)a->grad_scale};
+                              a->advantages, a->adv_per_row ? 0 : a->ld_adv, pc, con, (typename Dt::raw*)a->dlogp, a->ld_dlogp, (int)rows, gpr, a->grad_scale};
     if (need == 0) {
       POLICY_LAUNCH(policy_small_kernel, dim3(1), dim3(1024), r, reduce, a->kl_coef, a->loss, a->stats);
       return;

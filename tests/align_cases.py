@@ -412,6 +412,28 @@ def case_not_a_number(device):
     assert loss.item() == 0.0 and not grad.cpu().any()
 
 
+def case_without_gradient(device):
+    """want_grad=False: no gradient, the same loss, log ratios and statistics -- in one launch and in several"""
+    g = torch.Generator().manual_seed(9)
+    for P, n, N, T in ((2, 40, 5, 7), (5, 9000, 70, 300)):
+        t, r, p = (torch.randn(2 * P, 4, n, generator=g).to(device) for _ in range(3))
+        lp, ref = (-torch.rand(N // 2 * 2, T, generator=g).to(device) for _ in range(2))
+        adv = torch.randn(N // 2 * 2, generator=g).to(device)
+        for f in (lambda w: ops.denoise_preference_loss(p, r, t, want_grad=w), lambda w: ops.preference_loss(lp, ref, want_grad=w),
+                  lambda w: ops.policy_loss(lp, adv, old_logp=ref, ref_logp=ref, kl_coef=0.1, want_grad=w),
+                  lambda w: ops.policy_loss(lp, adv, reduce="row", want_grad=w)):
+            a, b = f(True), f(False)
+            assert b[1] is None and a[1].abs().sum().item() > 0 and torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+    # the sampler's four-dimensional latents, and an infinite bound
+    x = torch.randn(3, 4, 16, 16, generator=g).to(device)
+    s = torch.full((3,), 0.5, device=device)
+    assert torch.equal(ops.transition_logprob(x, x * 0.5, s), ops.transition_logprob(x.flatten(1), (x * 0.5).flatten(1), s))
+    assert ops.transition_logprob_bwd(x, x * 0.5, s, s).shape == x.shape
+    before = x.clone()
+    norm = ops.GradSet([x]).clip(float("inf"))
+    assert torch.equal(x, before) and abs(norm.item() - before.double().norm().item()) <= 2 * U * norm.item()
+
+
 def case_infinite_margins(device):
     """a sample the policy or the reference rules out: the pair's loss is 0 or infinite, its gradient that of the limit, and no 0 times infinity"""
     inf = float("inf")

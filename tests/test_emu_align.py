@@ -82,6 +82,10 @@ def test_not_a_number():
     A.case_not_a_number("cpu")
 
 
+def test_without_gradient():
+    A.case_without_gradient("cpu")
+
+
 def test_infinite_margins():
     A.case_infinite_margins("cpu")
 

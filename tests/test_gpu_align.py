@@ -39,7 +39,7 @@ def test_preference(P, T, kw):
                                     (2, 40, dict(with_old=False, kl=0.2)), (30, 1700, dict(with_ref=True, i64=True, ragged=True, reduce="row")),
                                     (5000, 1, dict(per_step=True, spread=3.0, kl=0.01)), (2, 300, dict(clip=(0.0, 0.0))), (5000, 7, dict(ragged=True, masked=True, reduce="row")),
                                     (40, 500, dict(clip=(0.9, float("inf")), kl=0.1, spread=1.0)), (600, 5000, dict(reduce="row", masked=True, kl=0.1, pad=3)),
-                                    (4, 50001, dict(reduce="row", masked=True, ragged=True)), (9000, 3, dict(reduce="row", masked=True)), (9000, 2, dict(per_step=True, pad=2, dtype="bf16")),
+                                    (4, 50001, dict(reduce="row", masked=True, ragged=True)), (1, 20000, dict(reduce="row", masked=True, kl=0.1)), (2, 3000, dict(grad_scale=3.3e4, dtype="f16")), (9000, 3, dict(reduce="row", masked=True)), (9000, 2, dict(per_step=True, pad=2, dtype="bf16")),
                                     (6000, 100, dict(ragged=True, i64=True)), (512, 2048, dict(kl=0.04)), (1, 100003, dict(masked=True, kl=0.04, per_step=True))])
 def test_policy(N, T, kw):
     A.case_policy("cuda", N, T, **kw)
@@ -73,6 +73,10 @@ def test_deterministic():
 
 def test_not_a_number():
     A.case_not_a_number("cuda")
+
+
+def test_without_gradient():
+    A.case_without_gradient("cuda")
 
 
 def test_infinite_margins():
