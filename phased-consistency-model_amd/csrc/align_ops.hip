@@ -102,7 +102,8 @@ __device__ __forceinline__ void pair_loss(const PairLoss p, double h, double* lo
     const double s = p.beta * h, e = exp(-fabs(s)), soft = log1p(e);             // -log sig(s) = soft + max(-s, 0)
     *loss = (1.0 - p.eps) * (soft + fmax(-s, 0.0));
     if (p.eps > 0.0) *loss += p.eps * (soft + fmax(s, 0.0));                      // (not 0 times infinity)
-    *slope = p.beta * ((s >= 0.0 ? 1.0 / (1.0 + e) : e / (1.0 + e)) - (1.0 - p.eps));
+    const double far = e / (1.0 + e), near = 1.0 / (1.0 + e);                     // sig(-|s|), sig(|s|): 1 - sig(|s|) has no digits left where s is large
+    *slope = p.beta * (p.eps * (s >= 0.0 ? near : far) - (1.0 - p.eps) * (s >= 0.0 ? far : near));
     if (!(s == s)) *loss = s;                                                     // fmax drops a NaN
   } else if (p.kind == PCM_PAIR_HINGE) {
     const double s = p.beta * h;

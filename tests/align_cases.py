@@ -526,3 +526,26 @@ def case_dense_orders(device):
     empty = ops.GradSet([torch.empty(0, device=device)])
     sumsq = torch.ones(1, dtype=torch.float64, device=device)
     assert empty.clip(1.0, sumsq=sumsq).item() == 0.0 and sumsq.item() == 0.0
+
+
+# ---- where terms cancel, overflow or reach a limit: bounds relative to the 64-bit value ----
+def case_separated_pairs(device):
+    """the slope of pairs that are far apart keeps its digits down to the smallest number of fp32: margins s = beta * h with beta = 1, so that the
+    margin itself is exact"""
+    for eps in (0.0, 0.1):
+        for s in (-60.0, -25.0, 0.0, 5.0, 17.0, 25.0, 30.0, 36.0, 38.0, 60.0, 85.0):
+            lp = torch.tensor([[s], [0.0]], device=device)
+            loss, grad, ratio = ops.preference_loss(lp, torch.zeros_like(lp), beta=1.0, label_smoothing=eps)
+            down = math.exp(-s) / (1 + math.exp(-s)) if s >= 0 else 1 / (1 + math.exp(s))      # sig(-s) and sig(s), each without a difference
+            up = math.exp(s) / (1 + math.exp(s)) if s < 0 else 1 / (1 + math.exp(-s))
+            want = eps * up - (1 - eps) * down
+            # fp64 throughout (its roundings, of what is subtracted, do not count), rounded once to the factor and once to the output
+            close(grad, torch.tensor([[want], [-want]], dtype=torch.float64), 3 * U * abs(want) + 16 * 2.0 ** -53 + 2.0 ** -149 if eps else 3 * U * abs(want), (eps, s))
+    # the same through the launches of many pairs
+    P = 200
+    s = torch.linspace(-20.0, 80.0, P).float()
+    lp = torch.cat([s, torch.zeros(P)])[:, None]
+    _, grad, _ = ops.preference_loss(lp.to(device), torch.zeros_like(lp).to(device), beta=1.0)
+    want = -torch.sigmoid(-s.double()) / P
+    close(grad[:P, 0], want, 4 * U * want.abs(), "many pairs")
+    close(grad[P:, 0], -want, 4 * U * want.abs(), "many pairs")

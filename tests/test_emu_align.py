@@ -96,3 +96,7 @@ def test_refusals():
 
 def test_dense_orders():
     A.case_dense_orders("cpu")
+
+
+def test_separated_pairs():
+    A.case_separated_pairs("cpu")

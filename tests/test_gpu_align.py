@@ -83,6 +83,10 @@ def test_infinite_margins():
     A.case_infinite_margins("cuda")
 
 
+def test_separated_pairs():
+    A.case_separated_pairs("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
