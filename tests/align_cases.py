@@ -549,3 +549,39 @@ def case_separated_pairs(device):
     want = -torch.sigmoid(-s.double()) / P
     close(grad[:P, 0], want, 4 * U * want.abs(), "many pairs")
     close(grad[P:, 0], -want, 4 * U * want.abs(), "many pairs")
+
+
+def case_far_reference(device):
+    """the KL term and its gradient, 1 - exp(d), where policy and reference are far apart, up to a reference that rules a place out (d = -inf) and a
+    policy that does (d = inf)"""
+    inf = float("inf")
+    for dtype in ("f32", "bf16", "f16"):
+        dt = DTYPES[dtype]
+        ds = torch.tensor([-inf, torch.finfo(dt).min, -3e4, -1e4, -300.0, -20.0, -10.0, -2.5, -0.75, -0.5, -0.25, -2.0 ** -9, 0.0, 2.0 ** -9, 0.25, 0.5, 0.75, 2.5, 10.0, inf],
+                          dtype=dt)
+        # in one launch (rows of one place, of three, of nine), in several, and a row to a workgroup
+        for rows, cols, reduce in ((1, 1, "sum"), (7, 3, "sum"), (3, 9, "sum"), (40, 500, "sum"), (32, 520, "row")):
+            for d0 in range(len(ds)) if cols == 1 else (0,):
+                ref = ds[(torch.arange(rows * cols) + d0) % len(ds)].view(rows, cols)
+                lp = torch.zeros(rows, cols, dtype=dt)
+                lp[ref == inf] = -inf                                        # the policy rules the place out: d = inf
+                ref[ref == inf] = 0.0
+                d = ref.double() - lp.double()
+                for kl, a in ((1.0, 0.0), (0.04, 1.0)):
+                    scale = float(rows * cols) if reduce == "row" else 1.0
+                    old = torch.zeros_like(lp)
+                    loss, grad, stats = ops.policy_loss(lp.to(device), torch.full((rows,), a, device=device), old_logp=old.to(device), ref_logp=ref.to(device),
+                                                        kl_coef=kl, reduce=reduce, grad_scale=scale)
+                    rise, r = torch.special.expm1(d), torch.exp(lp.double())
+                    want = -a * r - kl * rise
+                    # the exponential's four half steps, the difference's one, the product's and the sum's one each; the weight's one
+                    tol = U * (6 * kl * torch.where(d.abs() < 0.5, rise.abs(), torch.exp(d)) + kl * rise.abs() + 4 * a * r + 3 * want.abs())
+                    if a:                                                    # (advantage 0 and lp = -inf: 0 * (-inf - 0), no number)
+                        close(grad, want, out_tol(want, tol, dt), (dtype, rows, cols, a, d0))
+                    else:
+                        fine = lp > -inf
+                        close(grad[fine.to(device)], want[fine], out_tol(want, tol, dt)[fine], (dtype, rows, cols, a, d0))
+                    kd = torch.where(d == inf, inf, rise - d)
+                    w = scale if reduce == "row" else 1.0
+                    t_kl = U * torch.where(d.abs() < 0.5, 16 * kd, 8 * torch.exp(d) + 3 * d.abs() + 2)
+                    close(stats[1].reshape(1), (kd.sum() / w).reshape(1), (t_kl.sum() / w + 9 * U * kd.sum() / w).reshape(1), "KL")

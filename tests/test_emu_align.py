@@ -100,3 +100,7 @@ def test_dense_orders():
 
 def test_separated_pairs():
     A.case_separated_pairs("cpu")
+
+
+def test_far_reference():
+    A.case_far_reference("cpu")

@@ -87,6 +87,10 @@ def test_separated_pairs():
     A.case_separated_pairs("cuda")
 
 
+def test_far_reference():
+    A.case_far_reference("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
