@@ -477,7 +477,7 @@ __device__ __forceinline__ void policy_place(const PolicyConst& c, const PolicyS
   if constexpr (KL) {
     float rise;
     kl_term(ref - lp, kl, &rise);
-    *slope -= c.kl * rise;
+    *slope -= c.kl * (c.kl != 0.f ? rise : 0.f);      // (coefficient 0: the KL is only watched, no 0 times infinity enters the gradient)
   }
 }
 #define POLICY_GROUP 4      /* places of a thread's group in every format (8 need 98 registers: half the waves, 59 us against 50 at 2048 x 8192) */
@@ -661,7 +661,7 @@ __device__ __forceinline__ void policy_part(const PolicyRows<Dt>& a, const Polic
   pcm_block_sums<NT>(sum, red);
 }
 __device__ __forceinline__ void policy_result(const double (&s)[POLICY_SUMS], double kl, float* loss, float* stats) {
-  loss[0] = (float)(s[POLICY_OBJ] + kl * s[POLICY_KL]);
+  loss[0] = (float)(kl != 0.0 ? s[POLICY_OBJ] + kl * s[POLICY_KL] : s[POLICY_OBJ]);
   stats[0] = (float)s[POLICY_OBJ]; stats[1] = (float)s[POLICY_KL]; stats[2] = (float)(s[POLICY_HELD] / fmax(s[POLICY_COUNT], 1.0)); stats[3] = (float)s[POLICY_COUNT];
 }
 __device__ __forceinline__ void policy_store(const double (&s)[POLICY_SUMS], double* part) {

@@ -585,3 +585,24 @@ def case_far_reference(device):
                     w = scale if reduce == "row" else 1.0
                     t_kl = U * torch.where(d.abs() < 0.5, 16 * kd, 8 * torch.exp(d) + 3 * d.abs() + 2)
                     close(stats[1].reshape(1), (kd.sum() / w).reshape(1), (t_kl.sum() / w + 9 * U * kd.sum() / w).reshape(1), "KL")
+
+
+def case_monitored_kl(device):
+    """kl_coef = 0 with a reference: the KL is in the statistics, loss and gradient are those of the call without reference, also where the KL is infinite"""
+    inf = float("inf")
+    for rows, cols, reduce in ((1, 1, "token"), (3, 9, "token"), (40, 500, "token"), (32, 520, "row"), (6000, 3, "sum")):
+        g = torch.Generator().manual_seed(rows)
+        lp = -torch.rand(rows, cols, generator=g)
+        old, adv = lp + 0.1 * torch.randn(rows, cols, generator=g), torch.randn(rows, generator=g)
+        for d in (1.0, 95.0, inf, -inf):
+            ref = lp.clone()
+            ref[0, 0] += d
+            lp, old, ref, adv = (t.to(device) for t in (lp, old, ref, adv))
+            with_ref = ops.policy_loss(lp, adv, old_logp=old, ref_logp=ref, kl_coef=0.0, reduce=reduce)
+            without = ops.policy_loss(lp, adv, old_logp=old, reduce=reduce)
+            assert torch.isfinite(without[0]).all() and torch.equal(with_ref[0], without[0]), (rows, cols, d)
+            assert torch.equal(with_ref[1], without[1]), (rows, cols, d)
+            kl = with_ref[2][1].item()
+            assert (kl == inf) if d != 1.0 else 0.0 < kl < 1.0, (rows, cols, d, kl)
+            assert torch.equal(with_ref[2][[0, 2, 3]], without[2][[0, 2, 3]])
+            lp, old, adv = lp.cpu(), old.cpu(), adv.cpu()

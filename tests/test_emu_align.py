@@ -104,3 +104,7 @@ def test_separated_pairs():
 
 def test_far_reference():
     A.case_far_reference("cpu")
+
+
+def test_monitored_kl():
+    A.case_monitored_kl("cpu")

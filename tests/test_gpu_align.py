@@ -91,6 +91,10 @@ def test_far_reference():
     A.case_far_reference("cuda")
 
 
+def test_monitored_kl():
+    A.case_monitored_kl("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
