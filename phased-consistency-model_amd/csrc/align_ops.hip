@@ -469,8 +469,8 @@ __device__ __forceinline__ void policy_place(const PolicyConst& c, const PolicyS
     const double e = (double)lp - (double)old;
     beyond = !s.zero && (s.neg ? e < c.log_under : e > c.log_over);
   }
-  // an advantage of zero adds nothing, also where exp leaves fp32 (x - x: 0, or the NaN of a NaN or an infinity)
-  const float ar = s.zero ? x - x : s.a * exp_of(x);
+  // an advantage of zero adds nothing, also where exp leaves fp32 or either policy rules the place out; a NaN stays one
+  const float ar = s.zero ? (x == x ? 0.f : x) : s.a * exp_of(x);
   *held = beyond;
   *obj = beyond ? s.held : -ar;
   *slope = beyond ? 0.f : -ar;

@@ -606,3 +606,19 @@ def case_monitored_kl(device):
             assert (kl == inf) if d != 1.0 else 0.0 < kl < 1.0, (rows, cols, d, kl)
             assert torch.equal(with_ref[2][[0, 2, 3]], without[2][[0, 2, 3]])
             lp, old, adv = lp.cpu(), old.cpu(), adv.cpu()
+
+
+def case_zero_advantage(device):
+    """an advantage of zero takes a place out of the objective, also where old or new policy rule it out; a NaN stays one"""
+    inf, nan = float("inf"), float("nan")
+    for rows, cols in ((1, 2), (5, 7), (40, 500)):
+        for lp0, old0, want in ((-inf, 0.0, 0.0), (0.0, -inf, 0.0), (200.0, -200.0, 0.0), (nan, 0.0, nan), (-inf, -inf, nan)):
+            lp, old, adv = torch.zeros(rows, cols), torch.zeros(rows, cols), torch.ones(rows, cols)
+            lp[0, 1], old[0, 1], adv[0, 1] = lp0, old0, 0.0
+            loss, grad, stats = ops.policy_loss(lp.to(device), adv.to(device), old_logp=old.to(device), reduce="sum")
+            wl = torch.tensor([-(rows * cols - 1.0) + want], dtype=torch.float64)
+            close(loss, wl, 0.0, ("loss", lp0, old0))
+            wg = torch.full((rows, cols), -1.0, dtype=torch.float64)
+            wg[0, 1] = want
+            close(grad, wg, 0.0, ("gradient", lp0, old0))
+            assert stats[2].item() == 0.0

@@ -108,3 +108,7 @@ def test_far_reference():
 
 def test_monitored_kl():
     A.case_monitored_kl("cpu")
+
+
+def test_zero_advantage():
+    A.case_zero_advantage("cpu")

@@ -95,6 +95,10 @@ def test_monitored_kl():
     A.case_monitored_kl("cuda")
 
 
+def test_zero_advantage():
+    A.case_zero_advantage("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
