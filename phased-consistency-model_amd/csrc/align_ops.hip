@@ -117,7 +117,8 @@ __device__ __forceinline__ void pair_loss(const PairLoss p, double h, double* lo
 }
 // A source of log ratios gives, for a range of a row: sums() -- what the thread adds to the row's sums; and grad() -- its part of the gradient, f being
 // the row's factor.  rho() and factor() turn a row's sums into its log ratio and into what multiplies the pair's slope in f.
-// Denoising errors: rho = -w k sum ((t - p)^2 - (t - r)^2);  d rho / d p = 2 w k (t - p)
+// Denoising errors: rho = -w k sum ((t - p)^2 - (t - r)^2);  d rho / d p = 2 w k (t - p).  The difference of the squares is summed as
+// (r - p) ((t - p) + (t - r)): its error shrinks with r - p, and predictions that agree give exactly 0, where squares formed apart cancel.
 template <typename Dt_>
 struct DenoiseRows {
   typedef Dt_ Dt;
@@ -140,7 +141,7 @@ struct DenoiseRows {
       [&](int u, long i, long left) {
         float e = 0.f;
 #pragma unroll
-        for (int j = 0; j < Dt::VEC; j++) { const float a = t[u][j] - p[u][j], b = t[u][j] - r[u][j]; e += a * a - b * b; }
+        for (int j = 0; j < Dt::VEC; j++) e += (r[u][j] - p[u][j]) * ((t[u][j] - p[u][j]) + (t[u][j] - r[u][j]));
         s += (double)e;
       });
     acc[0] = s;

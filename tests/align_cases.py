@@ -622,3 +622,27 @@ def case_zero_advantage(device):
             wg[0, 1] = want
             close(grad, wg, 0.0, ("gradient", lp0, old0))
             assert stats[2].item() == 0.0
+
+
+def case_student_near_base(device):
+    """the log ratios of a student close to its frozen base, as at the start of every run: exactly 0 where the predictions agree, and with an error that
+    shrinks with their distance"""
+    for P, n in ((1, 16384), (8, 500), (200, 300), (2, 20001)):
+        for dtype in ("f32", "bf16", "f16"):
+            dt = DTYPES[dtype]
+            g = torch.Generator().manual_seed(n)
+            t = torch.randn(2 * P, n, generator=g).to(dt)
+            r = (t.float() + 0.3 * torch.randn(2 * P, n, generator=g)).to(dt)
+            for away in (0.0, 1e-6, 1e-5, 1e-3):
+                p = (r.float() + away * torch.randn(2 * P, n, generator=g)).to(dt)
+                beta = 200.0
+                loss, grad, ratio = ops.denoise_preference_loss(p.to(device), r.to(device), t.to(device), beta=beta)
+                a, b, d = t.double() - p.double(), t.double() - r.double(), r.double() - p.double()
+                want = -(d * (a + b)).mean(1)
+                # differences, their sum and the product one rounding each, up to eight fp32 additions
+                tol = 12 * U * (d.abs() * (a.abs() + b.abs())).mean(1)
+                close(ratio, want, tol + U * want.abs(), (P, n, dtype, away))
+                s = beta * (want[:P] - want[P:])
+                close(loss, -torch.nn.functional.logsigmoid(s).mean().reshape(1), beta * (tol[:P] + tol[P:]).mean() + 2 * U, (P, n, dtype, away))
+                if away == 0.0:
+                    assert not ratio.cpu().any()

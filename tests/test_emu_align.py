@@ -112,3 +112,7 @@ def test_monitored_kl():
 
 def test_zero_advantage():
     A.case_zero_advantage("cpu")
+
+
+def test_student_near_base():
+    A.case_student_near_base("cpu")

@@ -99,6 +99,10 @@ def test_zero_advantage():
     A.case_zero_advantage("cuda")
 
 
+def test_student_near_base():
+    A.case_student_near_base("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
