@@ -234,10 +234,10 @@ struct TokenRows {
         pcm_ld_group<Dt>(lr + i, left, a[u]); pcm_ld_group<Dt>(rr + i, left, b[u]);
       },
       [&](int u, long i, long left) {
-        float e = 0.f;
+        // (each into the fp64 sum: a few of the lowest number, which stands for a logarithm of 0, leave fp32.  512 pairs of 4096 fp32 in 21.8 us against
+        // 21.7 with a group's 4 added in fp32 first, of 8192 bf16, 8 to a group, in 23.2 against 22.9)
 #pragma unroll
-        for (int j = 0; j < Dt::VEC; j++) { e += in[u] >> j & 1u ? a[u][j] - b[u][j] : 0.f; cnt += in[u] >> j & 1u; }
-        s += (double)e;
+        for (int j = 0; j < Dt::VEC; j++) { s += (double)(in[u] >> j & 1u ? a[u][j] - b[u][j] : 0.f); cnt += in[u] >> j & 1u; }
       });
     acc[0] = s; acc[1] = (double)cnt;
   }

@@ -646,3 +646,19 @@ def case_student_near_base(device):
                 close(loss, -torch.nn.functional.logsigmoid(s).mean().reshape(1), beta * (tol[:P] + tol[P:]).mean() + 2 * U, (P, n, dtype, away))
                 if away == 0.0:
                     assert not ratio.cpu().any()
+
+
+def case_lowest_reference(device):
+    """log-probabilities of the format's lowest number at places that count: their sums leave fp32 but not the margin of a pair whose rows both hold them"""
+    for dtype in ("f32", "bf16"):
+        dt = DTYPES[dtype]
+        low = torch.finfo(dt).min
+        for P, T in ((1, 2), (2, 8), (3, 1500), (100, 400)):
+            lp, ref = torch.zeros(2 * P, T, dtype=dt), torch.full((2 * P, T), low, dtype=dt)
+            for reduce in ("mean", "sum"):
+                loss, grad, ratio = ops.preference_loss(lp.to(device), ref.to(device), beta=0.5, reduce=reduce)
+                close(loss, torch.tensor([math.log(2.0)], dtype=torch.float64), 2 * U, (dtype, P, T, reduce))
+                close(ratio, torch.full((2 * P,), -low if reduce == "mean" else math.inf).double(), 2 * U * -low, (dtype, P, T, reduce))
+                g = -0.25 / P / (T if reduce == "mean" else 1)
+                want = torch.cat([torch.full((P, T), g), torch.full((P, T), -g)]).double()
+                close(grad, want, out_tol(want, 2 * U * want.abs(), dt), (dtype, P, T, reduce))

@@ -116,3 +116,7 @@ def test_zero_advantage():
 
 def test_student_near_base():
     A.case_student_near_base("cpu")
+
+
+def test_lowest_reference():
+    A.case_lowest_reference("cpu")

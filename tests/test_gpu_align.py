@@ -103,6 +103,10 @@ def test_student_near_base():
     A.case_student_near_base("cuda")
 
 
+def test_lowest_reference():
+    A.case_lowest_reference("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
