@@ -401,15 +401,15 @@ static void pair_launch(const R& r, double* part, const PairLoss& pl, double gsc
     return;
   }
   const RowCut c = row_cut(rows, n, R::Dt::VEC);
-  const unsigned nb = row_cut_blocks(c, rows), ng = r.wants_grad() ? nb + 1 : 1;
   const bool apart = pairs > PAIR_LOSS_ONE;
+  const unsigned nb = row_cut_blocks(c, rows), ng = r.wants_grad() ? nb + 1 : (apart ? 0 : 1);      // workgroups of the gradient, and the one of the loss
   float* at_once = apart ? nullptr : loss;
   if (c.team == 64) {
     PCM_LAUNCH((pair_sums_kernel<R, 64>), dim3(nb), dim3(256), 0, stream, r, part, rows, n, c.chunks, c.len);
-    PCM_LAUNCH((pair_grad_kernel<R, 64>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, at_once, log_ratio, pairs, n, c.chunks, c.len);
+    if (ng) PCM_LAUNCH((pair_grad_kernel<R, 64>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, at_once, log_ratio, pairs, n, c.chunks, c.len);
   } else {
     PCM_LAUNCH((pair_sums_kernel<R, 256>), dim3(nb), dim3(256), 0, stream, r, part, rows, n, c.chunks, c.len);
-    PCM_LAUNCH((pair_grad_kernel<R, 256>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, at_once, log_ratio, pairs, n, c.chunks, c.len);
+    if (ng) PCM_LAUNCH((pair_grad_kernel<R, 256>), dim3(ng), dim3(256), 0, stream, r, (const double*)part, pl, gscale, at_once, log_ratio, pairs, n, c.chunks, c.len);
   }
   if (apart) {
     double* loss_part = part + rows * c.chunks * R::SUMS;

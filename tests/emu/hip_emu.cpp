@@ -105,7 +105,9 @@ hipError_t set_max_dyn_lds(const void* fn, int bytes) {
   return 0;
 }
 
+static long g_launches = 0;      // kernels launched so far (pcm_emu_launches)
 void launch(const void* fn, dim3 grid, dim3 block, size_t smem, std::function<void()> body) {
+  g_launches++;
   {
     auto it = g_max_dyn.find(fn);
     const size_t lim = it == g_max_dyn.end() ? LDS_DEFAULT_DYN : std::max(it->second, LDS_DEFAULT_DYN);
@@ -189,6 +191,9 @@ void launch(const void* fn, dim3 grid, dim3 block, size_t smem, std::function<vo
   g_cur = nullptr;
 }
 }  // namespace pcm_emu
+
+// how many kernels were launched: the difference over a call shows a launch that nothing needs
+extern "C" long pcm_emu_launches() { return pcm_emu::g_launches; }
 
 // self-test hook for tests/test_emu_kernels.py::test_emulator_enforces_launch_limits: launch an empty kernel with the given dynamic LDS
 // request / block size (optionally after raising the kernel's dynamic-LDS cap) and return what hipGetLastError would report

@@ -120,3 +120,17 @@ def test_student_near_base():
 
 def test_lowest_reference():
     A.case_lowest_reference("cpu")
+
+
+def test_launches_of_the_preference_loss():
+    """a call launches what it needs: few elements one kernel; partial sums and gradient two; the loss of many pairs two of its own, and then none for a
+    gradient that is not asked for"""
+    import ctypes
+    from pcm_amd import ops
+    count = capi.lib().dll.pcm_emu_launches
+    count.restype, count.argtypes = ctypes.c_long, []
+    for P, T, want_grad, launches in ((4, 50, True, 1), (4, 50, False, 1), (100, 400, True, 2), (100, 400, False, 2), (2500, 2, True, 4), (2500, 2, False, 3)):
+        lp = -torch.rand(2 * P, T)
+        before = count()
+        ops.preference_loss(lp, torch.zeros_like(lp), want_grad=want_grad)
+        assert count() - before == launches, (P, T, want_grad)
