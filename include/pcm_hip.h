@@ -471,7 +471,8 @@ int pcm_cast_bf16_f32(const void* x, float* y, long n, void* stream);
 /* ---- alignment of the distilled student (abi >= 6): preference losses, clipped policy loss, transition log-probability, gradient norm ----
  * Element formats of these calls are named per call and do not depend on the build's 16-bit format.  Elements are formed in fp32, sums are
  * carried in fp64 in a fixed order (no atomics): results are bitwise the same run to run.  `workspace` is 8-byte aligned caller scratch of at
- * least the matching *_workspace_bytes; it is only used between the launches of the call.  Gradients are those of grad_scale * loss. */
+ * least the matching *_workspace_bytes; it is only used between the launches of the call.  Gradients are those of grad_scale * loss.
+ * At most 2^24 rows (2^23 pairs), two less where rows of more than 1024 elements take a workgroup each (not in pcm_policy_loss). */
 #define PCM_DT_F32 0
 #define PCM_DT_BF16 1
 #define PCM_DT_F16 2

@@ -743,7 +743,9 @@ __global__ __launch_bounds__(1024) void policy_small_kernel(PolicyRows<Dt> a, in
 
 // ---- entry points ----
 #define AL_MAX_LD 4294967296L
-#define AL_MAX_ROWS 16777216L       /* 64 chunks of a row at the most: a grid stays below 2^31 workgroups */
+#define AL_MAX_ROWS 16777216L
+// a launch has fewer than 2^32 threads: long rows take a workgroup of 256 each (several only where rows are few), and the pairs' loss one more
+static bool rows_ok(long rows, long n) { return rows > 0 && rows <= AL_MAX_ROWS && (n <= 1024 || rows <= AL_MAX_ROWS - 2); }
 // the forward pass takes a row to a workgroup of 1024 where rows are too few for one chunk each but short enough: one launch instead of two.  16 rows of
 // 16384: 4.2 us against 3.1 + 2.5 and 4 us less host time; one row of 65536 among others 12 us against 16, of 131072 alone 28 against 26
 static RowCut transition_cut(long rows, long n, int vec) {
@@ -758,7 +760,7 @@ extern "C" size_t pcm_transition_logprob_workspace_bytes(long rows, long n) {
 }
 extern "C" int pcm_transition_logprob(const void* x, const void* mean, const float* std, int dtype, int mean_reduce, float* logp, long rows, long n,
                                       void* workspace, size_t workspace_bytes, void* stream) {
-  PCM_CHECK(x && mean && std && logp && pcm_dt_ok(dtype) && rows > 0 && rows <= AL_MAX_ROWS && n > 0, PCM_EINVAL, "pcm_transition_logprob: null/empty or unknown format");
+  PCM_CHECK(x && mean && std && logp && pcm_dt_ok(dtype) && n > 0 && rows_ok(rows, n), PCM_EINVAL, "pcm_transition_logprob: null/empty, too many rows or unknown format");
   const size_t need = pcm_transition_logprob_workspace_bytes(rows, n);
   PCM_CHECK(need == 0 || (workspace && ((uintptr_t)workspace % 8) == 0 && workspace_bytes >= need), PCM_EINVAL,
             "pcm_transition_logprob: workspace too small or not 8-byte aligned");
@@ -778,8 +780,8 @@ extern "C" int pcm_transition_logprob(const void* x, const void* mean, const flo
 }
 extern "C" int pcm_transition_logprob_bwd(const void* x, const void* mean, const float* std, const float* dlogp, int dtype, int mean_reduce, void* dmean,
                                           long rows, long n, void* stream) {
-  PCM_CHECK(x && mean && std && dlogp && dmean && pcm_dt_ok(dtype) && rows > 0 && rows <= AL_MAX_ROWS && n > 0, PCM_EINVAL,
-            "pcm_transition_logprob_bwd: null/empty or unknown format");
+  PCM_CHECK(x && mean && std && dlogp && dmean && pcm_dt_ok(dtype) && n > 0 && rows_ok(rows, n), PCM_EINVAL,
+            "pcm_transition_logprob_bwd: null/empty, too many rows or unknown format");
   pcm_with_dtype(dtype, [&](auto dt) {
     typedef decltype(dt) Dt;
     typedef const typename Dt::raw* cp;
@@ -792,9 +794,9 @@ extern "C" int pcm_transition_logprob_bwd(const void* x, const void* mean, const
   return pcm_post_launch("pcm_transition_logprob_bwd");
 }
 
-static int pair_args_ok(const char* who, int dtype, long pairs, double beta, int kind, double eps) {
+static int pair_args_ok(const char* who, int dtype, long pairs, long n, double beta, int kind, double eps) {
   PCM_CHECK(pcm_dt_ok(dtype), PCM_EINVAL, "%s: unknown element format %d", who, dtype);
-  PCM_CHECK(pairs > 0 && pairs <= AL_MAX_ROWS / 2, PCM_EINVAL, "%s: number of pairs %ld", who, pairs);
+  PCM_CHECK(pairs > 0 && pairs <= AL_MAX_ROWS && rows_ok(2 * pairs, n), PCM_EINVAL, "%s: number of pairs %ld", who, pairs);
   PCM_CHECK(beta > 0.0 && beta < 1e30, PCM_EINVAL, "%s: beta must be positive and finite", who);
   PCM_CHECK(kind == PCM_PAIR_SIGMOID || kind == PCM_PAIR_HINGE || kind == PCM_PAIR_SQUARE, PCM_EINVAL, "%s: unknown kind %d", who, kind);
   PCM_CHECK(eps >= 0.0 && eps < 0.5 && (eps == 0.0 || kind == PCM_PAIR_SIGMOID), PCM_EINVAL, "%s: label smoothing must be in [0, 0.5) and needs the sigmoid kind", who);
@@ -803,7 +805,7 @@ static int pair_args_ok(const char* who, int dtype, long pairs, double beta, int
 extern "C" size_t pcm_denoise_preference_loss_workspace_bytes(long pairs, long n) { return pairs > 0 && n > 0 ? pair_ws_bytes(2 * pairs, n, DenoiseRows<DtF32>::SUMS) : 0; }
 extern "C" int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a, void* stream) {
   PCM_CHECK(a && a->pred && a->ref && a->target && a->loss && a->log_ratio && a->n > 0, PCM_EINVAL, "pcm_denoise_preference_loss: null/empty");
-  const int rc = pair_args_ok("pcm_denoise_preference_loss", a->dtype, a->pairs, a->beta, a->kind, a->label_smoothing);
+  const int rc = pair_args_ok("pcm_denoise_preference_loss", a->dtype, a->pairs, a->n, a->beta, a->kind, a->label_smoothing);
   if (rc != PCM_OK) return rc;
   const size_t need = pcm_denoise_preference_loss_workspace_bytes(a->pairs, a->n);
   PCM_CHECK(need == 0 || (a->workspace && ((uintptr_t)a->workspace % 8) == 0 && a->workspace_bytes >= need), PCM_EINVAL,
@@ -821,7 +823,7 @@ extern "C" int pcm_denoise_preference_loss(const pcm_denoise_preference_args* a,
 extern "C" size_t pcm_preference_loss_workspace_bytes(long pairs, long cols) { return pairs > 0 && cols > 0 ? pair_ws_bytes(2 * pairs, cols, TokenRows<DtF32>::SUMS) : 0; }
 extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   PCM_CHECK(a && a->logp && a->ref_logp && a->loss && a->log_ratio && a->cols > 0, PCM_EINVAL, "pcm_preference_loss: null/empty");
-  const int rc = pair_args_ok("pcm_preference_loss", a->dtype, a->pairs, a->beta, a->kind, a->label_smoothing);
+  const int rc = pair_args_ok("pcm_preference_loss", a->dtype, a->pairs, a->cols, a->beta, a->kind, a->label_smoothing);
   if (rc != PCM_OK) return rc;
   PCM_CHECK(a->ld_logp >= a->cols && a->ld_ref >= a->cols && (!a->mask || a->ld_mask >= a->cols) && (!a->dlogp || a->ld_dlogp >= a->cols), PCM_EINVAL,
             "pcm_preference_loss: row stride below the row length");

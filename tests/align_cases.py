@@ -662,3 +662,25 @@ def case_lowest_reference(device):
                 g = -0.25 / P / (T if reduce == "mean" else 1)
                 want = torch.cat([torch.full((P, T), g), torch.full((P, T), -g)]).double()
                 close(grad, want, out_tol(want, 2 * U * want.abs(), dt), (dtype, P, T, reduce))
+
+
+def case_too_many_rows(device):
+    """a launch has fewer than 2^32 threads: rows that would need more are refused before anything is read or launched"""
+    import ctypes as C
+    from pcm_amd import capi
+    x = torch.zeros(64, device=device)
+    p = x.data_ptr()
+    lib = capi.lib()
+    for rows, n in ((1 << 24, 2000), ((1 << 24) - 1, 2000), ((1 << 24) + 1, 1), (1 << 40, 1), (1 << 62, 2000)):
+        with pytest.raises(RuntimeError):
+            lib.call("pcm_transition_logprob", p, p, p, 0, 1, p, rows, n, p, 1 << 50, None)
+        with pytest.raises(RuntimeError):
+            lib.call("pcm_transition_logprob_bwd", p, p, p, p, 0, 1, p, rows, n, None)
+    for pairs, n in ((1 << 23, 2000), ((1 << 23) + 1, 1), (1 << 40, 1), (1 << 62, 2000)):
+        a = capi.DenoisePreferenceArgs(p, p, p, None, None, p, p, p, 1 << 50, pairs, n, 1.0, 0.0, 1.0, 0, 0, 0)
+        with pytest.raises(RuntimeError):
+            lib.call("pcm_denoise_preference_loss", C.byref(a), None)
+        a = capi.PreferenceArgs(p, p, None, None, None, p, p, p, 1 << 50, pairs, n, n, n, 0, n, 1.0, 0.0, 1.0, 0, 0, 0, 0)
+        with pytest.raises(RuntimeError):
+            lib.call("pcm_preference_loss", C.byref(a), None)
+    assert not x.cpu().any()

@@ -94,7 +94,7 @@ static void trampoline() {
 }
 
 // gfx950 launch limits (MI355X_MICROARCH.md): 160 KiB of LDS per CU / workgroup, of which a kernel may use more than 64 KiB of DYNAMIC
-// LDS only after hipFuncSetAttribute(MaxDynamicSharedMemorySize) raised its limit; 1024 threads per block; grid.y/z <= 65535.
+// LDS only after hipFuncSetAttribute(MaxDynamicSharedMemorySize) raised its limit; 1024 threads per block; grid.y/z <= 65535; fewer than 2^32 threads along x.
 // (static __shared__ arrays are host statics here and not counted: tests/test_codeobj_limits.py checks them on the gfx950 code object.)
 hipError_t g_last_error = 0;
 static std::map<const void*, size_t> g_max_dyn;
@@ -113,7 +113,7 @@ void launch(const void* fn, dim3 grid, dim3 block, size_t smem, std::function<vo
     const size_t lim = it == g_max_dyn.end() ? LDS_DEFAULT_DYN : std::max(it->second, LDS_DEFAULT_DYN);
     const unsigned long nthr = (unsigned long)block.x * block.y * block.z;
     if (smem > lim || smem > LDS_PER_CU || nthr == 0 || nthr > 1024 || grid.x == 0 || grid.y == 0 || grid.z == 0 || grid.y > 65535 ||
-        grid.z > 65535 || grid.x > 2147483647u) {
+        grid.z > 65535 || grid.x > 2147483647u || (unsigned long)grid.x * block.x >= (1ul << 32)) {
       fprintf(stderr, "pcm_emu: launch REJECTED (gfx950 limits): dynamic LDS %zu B (limit %zu), block %lu, grid (%u,%u,%u)\n", smem, lim, nthr,
               grid.x, grid.y, grid.z);
       g_last_error = hipErrorInvalidValue;

@@ -134,3 +134,7 @@ def test_launches_of_the_preference_loss():
         before = count()
         ops.preference_loss(lp, torch.zeros_like(lp), want_grad=want_grad)
         assert count() - before == launches, (P, T, want_grad)
+
+
+def test_too_many_rows():
+    A.case_too_many_rows("cpu")

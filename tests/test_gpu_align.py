@@ -107,6 +107,10 @@ def test_lowest_reference():
     A.case_lowest_reference("cuda")
 
 
+def test_too_many_rows():
+    A.case_too_many_rows("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
