@@ -684,3 +684,22 @@ def case_too_many_rows(device):
         with pytest.raises(RuntimeError):
             lib.call("pcm_preference_loss", C.byref(a), None)
     assert not x.cpu().any()
+
+
+def case_transition_scales(device):
+    """deviations far from 1: squares and the gradient's factor leave fp32 before their results do"""
+    for B, n, dtype in ((4, 40, "f32"), (4, 3000, "bf16"), (4, 70000, "f32"), (2, 140000, "bf16")):
+        dt = DTYPES[dtype]
+        g = torch.Generator().manual_seed(n)
+        for s, dl in ((1e-22, 1.0), (1e-19, 1e-3), (1e18, 1e-10), (1e25, 1e20)):
+            std = torch.full((B,), s)
+            x = (std[:, None] * torch.randn(B, n, generator=g)).to(dt)
+            mean, dlogp = torch.zeros(B, n, dtype=dt), torch.full((B,), dl)
+            sd, d = std.double()[:, None], x.double()
+            for reduce, k in (("mean", 1.0 / n), ("sum", 1.0)):
+                args = [t.to(device) for t in (x, mean, std)]
+                want = torch.distributions.Normal(mean.double(), sd.expand_as(d)).log_prob(d).sum(1) * k
+                # differences exact here, all else in fp64
+                close(ops.transition_logprob(*args, reduce=reduce), want, 2 * U * want.abs(), (B, n, s, reduce))
+                want = -dlogp.double()[:, None] * k * (mean.double() - d) / (sd * sd)
+                close(ops.transition_logprob_bwd(*args, dlogp.to(device), reduce=reduce), want, out_tol(want, 2 * U * want.abs(), dt), (B, n, s, reduce))

@@ -138,3 +138,7 @@ def test_launches_of_the_preference_loss():
 
 def test_too_many_rows():
     A.case_too_many_rows("cpu")
+
+
+def test_transition_scales():
+    A.case_transition_scales("cpu")

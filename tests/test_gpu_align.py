@@ -111,6 +111,10 @@ def test_too_many_rows():
     A.case_too_many_rows("cuda")
 
 
+def test_transition_scales():
+    A.case_transition_scales("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
