@@ -703,3 +703,37 @@ def case_transition_scales(device):
                 close(ops.transition_logprob(*args, reduce=reduce), want, 2 * U * want.abs(), (B, n, s, reduce))
                 want = -dlogp.double()[:, None] * k * (mean.double() - d) / (sd * sd)
                 close(ops.transition_logprob_bwd(*args, dlogp.to(device), reduce=reduce), want, out_tol(want, 2 * U * want.abs(), dt), (B, n, s, reduce))
+
+
+def case_sampler_transition(device):
+    """the stochastic flow-matching sampler's step from sigma to sigma_next as a transition: mean (1 - sigma_next) (x - sigma v), deviation sigma_next; the
+    gradient by the model's output v follows with the factor -(1 - sigma_next) sigma"""
+    from pcm_amd.fm import PCMFMSampler
+    g = torch.Generator().manual_seed(3)
+    sampler = PCMFMSampler(shift=3.0, stochastic=True)
+    sampler.set_timesteps(4)
+    x = torch.randn(2, 4, 8, 8, generator=g).to(device)
+    for t, s, s_next in zip(sampler.timesteps, sampler.sigmas_[:-1].tolist(), sampler.sigmas_[1:].tolist()):
+        v, noise = (torch.randn(x.shape, generator=g).to(device) for _ in range(2))
+        out = sampler.step(v, t, x, noise=noise)
+        mean = (1.0 - s_next) * (x - s * v)
+        if s_next == 0.0:                            # the last step draws nothing: no density
+            close(out, mean.cpu(), 8 * U * (x.abs() + v.abs()).cpu().double(), "last step")
+            break
+        close(out, (mean + s_next * noise).cpu(), 8 * U * (x.abs() + v.abs() + noise.abs()).cpu().double(), "step")
+        std = torch.full((2,), s_next, device=device)
+        logp = ops.transition_logprob(out, mean, std)
+        dlogp = torch.tensor([0.5, -2.0], device=device)
+        dv = -(1.0 - s_next) * s * ops.transition_logprob_bwd(out, mean, std, dlogp)
+        v64 = v.double().cpu().requires_grad_()
+        m64 = (1.0 - s_next) * (x.double().cpu() - s * v64)
+        want = torch.distributions.Normal(m64, s_next).log_prob(out.double().cpu()).flatten(1).mean(1)
+        (want * dlogp.double().cpu()).sum().backward()
+        # mean and step are rounded to fp32: up to eight half steps of the largest of their terms, divided by the deviation
+        off = 16 * U * (x.abs() + v.abs() + noise.abs()).double().cpu() / s_next
+        z = ((out.double().cpu() - m64) / s_next).detach()
+        close(logp, want.detach(), (z.abs() * off + off ** 2).flatten(1).mean(1) + 2 * U * want.detach().abs(), "log-probability")
+        n = x[0].numel()
+        tol = dlogp.double().cpu().abs()[:, None, None, None] * s * (1.0 - s_next) / s_next / n * off
+        close(dv, v64.grad, tol + 8 * U * v64.grad.abs(), "gradient by the model's output")
+        x = out

@@ -142,3 +142,7 @@ def test_too_many_rows():
 
 def test_transition_scales():
     A.case_transition_scales("cpu")
+
+
+def test_sampler_transition():
+    A.case_sampler_transition("cpu")

@@ -115,6 +115,10 @@ def test_transition_scales():
     A.case_transition_scales("cuda")
 
 
+def test_sampler_transition():
+    A.case_sampler_transition("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
