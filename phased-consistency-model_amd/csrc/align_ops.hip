@@ -4,8 +4,11 @@
 // which is why its exponentials are counted), small ones by their launches: about 4 us of host time each.  Times below are of one MI355X, whose
 // large copies run at 5.1 TB/s and whose reads alone reach 6.8.
 //
-// Elements are formed in fp32; every sum over elements, rows or tokens is carried in fp64 and in an order fixed by the launch (partial sums in the
-// caller's workspace, added up by index), so results are bitwise the same run to run.
+// Elements are formed in fp32 (squares and factors of a transition in fp64); every sum over elements, rows or tokens is carried in fp64 and in an order fixed
+// by the launch (partial sums in the caller's workspace, added up by index), so results are bitwise the same run to run.  Two kernels add a thread's group of
+// elements in fp32 first, where a sum that leaves fp32 takes terms no run comes by: the denoising errors (4 or 8; terms of 1e38 need predictions of 1e19) and
+// the policy loss (4; a ratio or exp(d) of 1e38).  Each into fp64 by itself cost the policy loss 0.6 us of 47.5 (2048 x 8192 fp32 with KL, ragged), 1.7 of 40
+// (bf16), and the denoising kernel of few elements registers that spilled.
 #include "dtype_dev.h"
 
 static inline int al_blocks(long n) { long b = (n + 255) / 256; return (int)(b > PCM_GRID_CAP(2048) ? PCM_GRID_CAP(2048) : (b < 1 ? 1 : b)); }
@@ -13,6 +16,12 @@ static inline int al_blocks(long n) { long b = (n + 255) / 256; return (int)(b >
 #define AL_U (16 / Dt::VEC)      /* groups of a thread in flight: 16 elements of every tensor */
 // how a launch cuts rows of n elements: teams of 64 (four rows to a workgroup) for short rows, else `chunks` workgroups of 256 per row, so that some
 // 4096 workgroups (two rounds of 8 per CU) share the work; at most 64 chunks, whose partial sums one wave adds up with one load per lane.
+// Measured on both sides, us of an eager call / of the same call replayed in a graph, where the host's share is gone:
+//   teams up to 1024 elements against 512: transition forward, 2048 rows of 1024 fp32 11.6 / 5.7 against 11.6 / 6.1, bf16 11.7 / 3.8 against 11.6 / 4.6;
+//   against 2048: 2048 rows of 1500 fp32 11.7 / 11.0 against 11.6 / 7.1, 64 rows of 1500 11.8 / 3.6 against 11.6 / 3.8; 100 pairs of 1500 18.7 / 7.2 against
+//   18.8 / 8.3, 1000 pairs 21.9 / 22.2 against 19.6 / 17.5: few rows want the workgroup, many the wave, and the limit looks at the length alone;
+//   64 chunks against 16: transition forward, one row of 2^20 fp32 15.5 / 6.8 against 15.6 / 7.9; one pair of 262144 18.7 / 14.2 against 18.8 / 13.3, 8 pairs
+//   28.0 / 28.2 against 22.8 / 22.9: of the pairs' loss, one thread adds up a pair's chunks one by one (pair_losses).
 struct RowCut { int team, chunks; long len; };
 #define ROW_TEAM_MAX 65536L
 static RowCut row_cut(long rows, long n, int vec) {
@@ -341,7 +350,9 @@ __global__ __launch_bounds__(256) void pair_loss_finish_kernel(const double* los
   if (threadIdx.x == 0) loss[0] = (float)(acc / (double)pairs);
 }
 // few elements: one workgroup takes all pairs in one launch -- a row to a wave, or to half of the waves where rows are long.  At the limit (one pair of
-// 16384 fp32) 14.2 us among others against 18.8 in two launches, alone 30.7 against 31.3; at twice as much alone 38 against 33
+// 16384 fp32) 14.2 us among others against 18.8 in two launches, alone 30.7 against 31.3; at twice as much alone 38 against 33.  The host's 4 us a launch
+// decide: in a replayed graph, where they are gone, one pair of 4096 takes 5.8 us either way, of 16384 10.0 against 7.4, 16 pairs of 1000 14.4 against 7.2; and 8
+// masked pairs of 2048 log-probabilities take 23.4 eager against 20.2
 #define PAIR_SMALL_ELEMENTS 32768L
 #define PAIR_SMALL_ROWS 128
 template <typename R>
@@ -422,7 +433,8 @@ static void pair_launch(const R& r, double* part, const PairLoss& pl, double gsc
 
 // ---- clipped policy loss with a KL term ----
 // e^x to about two steps: 2^t with t = x log2 e, the product's rounding error e carried along as the factor 1 + e ln 2 (v_exp_f32 alone would be off by
-// |x| half steps).  Half the instructions of expf; results below 2^-126 come out as 0.
+// |x| half steps).  Half the instructions of expf; results below 2^-126 come out as 0: a ratio or an exp(d) that small adds less than the last digit of
+// anything it stands beside.
 __device__ __forceinline__ float exp_of(float x) {
   const float hi = 1.44269502162933349609375f, lo = 1.92596299112661746887e-8f;      // log2 e in two fp32 numbers
   const float t = x * hi, e = fmaf(x, lo, fmaf(x, hi, -t)), r = PCM_EXP2F(t);
@@ -710,8 +722,9 @@ __global__ __launch_bounds__(256) void policy_finish_kernel(const double* part, 
   pcm_block_sums<256>(s, red);
   if (threadIdx.x == 0) policy_result(s, kl, loss, stats);
 }
-// few places: one workgroup counts, forms loss and gradient, and adds up, in one launch.  At the limit (64 x 256 bf16, masked) 17.7 us among others against
-// 24.6 in three launches, alone 39 against 36; at twice as much 23.2 against 24.5 and 47 against 36
+// few places: one workgroup counts, forms loss and gradient, and adds up, in one launch.  At the limit (64 x 256 bf16, masked) 17.2 us among others against
+// 23.9 in three launches, alone 39 against 36; at twice as much 22.4 against 24.1 and 47 against 36.  In a replayed graph, without the host's share, 8 x 4 takes 6.9
+// against 9.5, 64 x 128 9.5 against 10.2, 64 x 256 15.0 against 10.3
 #define POLICY_SMALL_PLACES 16384
 #define POLICY_SMALL_ROWS 2048
 template <bool KL, bool NARROW, typename Dt>
@@ -843,7 +856,10 @@ extern "C" int pcm_preference_loss(const pcm_preference_args* a, void* stream) {
   return pcm_post_launch("pcm_preference_loss");
 }
 static bool policy_small(long rows, long cols) { return rows <= POLICY_SMALL_ROWS && rows * cols <= POLICY_SMALL_PLACES; }
-// a workgroup to a row: rows long enough to keep it busy, and enough of them for the chip or none too long for one
+// a workgroup to a row: rows long enough to keep it busy, and enough of them for the chip or none too long for one.  Masked fp32 with KL, us eager / replayed,
+// by row against a launch for the weights and one over all groups: 2048 x 256 21.4 / 13.2 against 24.1 / 10.6, 2048 x 500 21.2 / 14.3 against 23.8 / 14.4, 512 x 520
+// 21.4 / 9.3 against 24.2 / 11.4, 40 x 4096 21.4 / 11.5 against 24.1 / 10.4, 40 x 5000 21.4 / 14.1 against 24.1 / 10.7, 300 x 8192 24.2 / 24.9 against 25.1 / 21.2,
+// 512 x 8192 26.2 / 26.5 against 25.5 / 25.9, 2048 x 8192 52.4 / 52.6 against 58.3 / 58.2
 static bool policy_by_row(int reduce, long rows, long cols) { return reduce == PCM_POLICY_ROW && cols >= 512 && (rows >= 512 || cols <= 4096); }
 #define POLICY_COUNT_PARTS 512
 // partial counts, or weights of rows
@@ -906,6 +922,8 @@ extern "C" int pcm_policy_loss(const pcm_policy_args* a, void* stream) {
         }
       } else if (reduce == PCM_POLICY_ROW) {
         pw.per_row = counts;
+        // (us replayed, a wave to a row against a workgroup: 2048 x 511 15.2 against 22.6, 300 x 4096 15.1 against 15.0, 500 x 8192 26.2 against 24.2, 8 x 32768 16.6
+        // against 10.3)
         if (a->cols <= 4096) PCM_LAUNCH(policy_weights_kernel<64>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, pc, rows, counts);
         else PCM_LAUNCH(policy_weights_kernel<1024>, dim3((unsigned)rows), dim3(1024), 0, stream, pc, rows, counts);
       }
