@@ -168,7 +168,10 @@ struct DenoiseRows {
       });
   }
   __device__ __forceinline__ double scale(long row) const { return k * (weight ? (double)weight[row] : 1.0); }
-  __device__ __forceinline__ double rho(long row, const double (&s)[SUMS]) const { return -s[0] * scale(row); }
+  __device__ __forceinline__ double rho(long row, const double (&s)[SUMS]) const {
+#pragma clang fp contract(off)      // (as in TokenRows)
+    return -s[0] * scale(row);
+  }
   __device__ __forceinline__ double factor(long row, const double (&s)[SUMS]) const { return 2.0 * scale(row); }
   bool wants_grad() const { return dpred != nullptr; }
 };
@@ -264,7 +267,12 @@ struct TokenRows {
       });
   }
   __device__ __forceinline__ double share(const double (&s)[SUMS]) const { return mean_reduce ? 1.0 / fmax(s[1], 1.0) : 1.0; }
-  __device__ __forceinline__ double rho(long row, const double (&s)[SUMS]) const { return s[0] * share(s); }
+  // Rounded before a pair's other log ratio is subtracted from it: contracted with that subtraction, one row's product would be exact and the other's not,
+  // and of equal rows the rounding error would be left -- 1e22 where the sums hold the lowest number of fp32.
+  __device__ __forceinline__ double rho(long row, const double (&s)[SUMS]) const {
+#pragma clang fp contract(off)
+    return s[0] * share(s);
+  }
   __device__ __forceinline__ double factor(long row, const double (&s)[SUMS]) const { return share(s); }
   bool wants_grad() const { return dlogp != nullptr; }
 };
