@@ -737,3 +737,18 @@ def case_sampler_transition(device):
         tol = dlogp.double().cpu().abs()[:, None, None, None] * s * (1.0 - s_next) / s_next / n * off
         close(dv, v64.grad, tol + 8 * U * v64.grad.abs(), "gradient by the model's output")
         x = out
+
+
+def case_without_gradient_16bit(device):
+    """want_grad=False in the 16-bit formats, over every launch form"""
+    for dtype in ("bf16", "f16"):
+        dt = DTYPES[dtype]
+        g = torch.Generator().manual_seed(4)
+        for P, T in ((2, 40), (5, 9000), (300, 130), (2500, 3)):
+            a, b, c = (torch.randn(2 * P, T, generator=g).to(dt).to(device) for _ in range(3))
+            adv = torch.randn(2 * P, generator=g).to(device)
+            mask = (torch.rand(2 * P, T, generator=g) < 0.7).to(device)
+            for f in (lambda w: ops.denoise_preference_loss(a, b, c, want_grad=w, beta=1.0), lambda w: ops.preference_loss(a, b, mask=mask, want_grad=w),
+                      lambda w: ops.policy_loss(a, adv, old_logp=b, ref_logp=c, mask=mask, kl_coef=0.1, want_grad=w), lambda w: ops.policy_loss(a, adv, old_logp=b, reduce="row", want_grad=w)):
+                x, y = f(True), f(False)
+                assert y[1] is None and torch.isfinite(x[0]).all() and torch.equal(x[0], y[0]) and torch.equal(x[2], y[2]), (dtype, P, T)

@@ -146,3 +146,7 @@ def test_transition_scales():
 
 def test_sampler_transition():
     A.case_sampler_transition("cpu")
+
+
+def test_without_gradient_16bit():
+    A.case_without_gradient_16bit("cpu")

@@ -119,6 +119,10 @@ def test_sampler_transition():
     A.case_sampler_transition("cuda")
 
 
+def test_without_gradient_16bit():
+    A.case_without_gradient_16bit("cuda")
+
+
 def test_refusals():
     A.case_refusals("cuda")
     from pcm_amd import ops
