@@ -526,6 +526,7 @@ int pcm_preference_loss(const pcm_preference_args* a, void* stream);
 /* Clipped policy loss with a KL term.  Per place that counts (mask / lengths as above), r = exp(logp - old_logp), d = ref_logp - logp:
  *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)  +  kl_coef * (exp(d) - d - 1)
  * clip_low in [0, 1), clip_high >= 0 or infinite.  old_logp NULL: the policy itself (r = 1 with its gradient).  A = advantages[row] (adv_per_row) or advantages[row][col].
+ * An advantage of 0 takes a place out of the objective; with kl_coef 0 a reference is only watched (stats), and loss and gradient are those without it.
  * Reduced by TOKEN: mean over all places;  ROW: mean over the rows of each row's mean (a row without places adds 0);  SUM.
  * stats fp32 [4] = {clipped objective, KL} (reduced the same way; loss = objective + kl_coef * KL), share of places held by the clip, places. */
 #define PCM_POLICY_TOKEN 0

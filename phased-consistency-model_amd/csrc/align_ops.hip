@@ -691,7 +691,7 @@ __device__ __forceinline__ void policy_store(const double (&s)[POLICY_SUMS], dou
     for (int k = 0; k < POLICY_SUMS; k++) part[(long)blockIdx.x * POLICY_SUMS + k] = s[k];
 }
 // (256, 8): 8 waves to a SIMD, so that all 2048 workgroups are resident at once; a workgroup takes consecutive groups (a strided grid reads 15 % slower).
-// 2048 x 8192 fp32 with old and reference log-probabilities: 268 MB in 50 us; with ragged rows, 194 MB, 42 us (without its arithmetic 13 % less).
+// 2048 x 8192 fp32 with old and reference log-probabilities: 268 MB in 50 us; with ragged rows, 194 MB, 43 us (without its arithmetic 13 % less).
 template <bool KL, bool NARROW, typename Dt>
 __global__ __launch_bounds__(256, 8) void policy_main_kernel(PolicyRows<Dt> a, PolicyWeight pw, double* part) {
   __shared__ double red[4 * POLICY_SUMS];
